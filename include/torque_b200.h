@@ -340,6 +340,92 @@ int tq_silu_mul(const void* gate_up, int64_t rows, int f, void* y, tq_stream_t s
 int tq_gemv(const void* weight, const void* x, int x_mode, const void* norm_weight, float eps,
             const void* residual, void* y, int n, int k, tq_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged 8-bit cache.  New in this build: the reference keeps one contiguous
+ * codebook cache per sequence (no counterpart).
+ *
+ * A pool holds pages of page_size (16, 32, 64 or 128) tokens of one layer:
+ *   k_pages, v_pages   [num_pages, kv_heads, page_size, head_dim] one-byte
+ *                      codes biased by 128 (1..255 stand for -127..127),
+ *                      16-byte aligned
+ *   k_scales, v_scales [num_pages, kv_heads] fp32; value = scale * (code - 128)
+ * A batch is ragged: sequence s holds lengths[s] tokens, brings rows
+ * [token_starts[s], token_starts[s+1]) of the call's row tensors (row s alone
+ * when token_starts is NULL) at positions lengths[s], lengths[s]+1, ..., and
+ * finds the page of position p at block_table[s*table_stride + p/page_size].
+ * lengths, token_starts and block_table are device memory, so a captured step
+ * follows them.  The kernels check what the host cannot: a page id outside
+ * the pool or a position past the table is not read or written, rows outside
+ * [0, rows) and more than max_new_tokens rows of one sequence are not
+ * processed.  seqs <= TQ_PAGED_MAX_SEQS.
+ * ------------------------------------------------------------------------- */
+
+#define TQ_PAGED_MAX_SEQS 2048
+
+typedef struct tq_paged_kv {
+  uint8_t* k_pages;
+  uint8_t* v_pages;
+  float* k_scales;
+  float* v_scales;
+  int64_t num_pages;
+  int32_t kv_heads;
+  int32_t page_size;
+  int32_t head_dim;
+} tq_paged_kv;
+
+typedef struct tq_paged_batch {
+  const int32_t* block_table;  /* [seqs, table_stride], table_width entries used */
+  const int32_t* lengths;      /* [seqs] tokens held before this call's rows */
+  const int32_t* token_starts; /* [seqs + 1] or NULL: one row each */
+  int64_t table_stride;
+  int64_t rows;                /* rows of the call's tensors */
+  int32_t table_width;
+  int32_t seqs;
+  int32_t max_new_tokens;      /* no sequence brings more rows than this */
+} tq_paged_batch;
+
+/* Appends the batch's rows to the pool, rotary positions applied on the way.
+ * qkv row r (x_dtype, row stride qkv_stride elements, rows 16-byte aligned)
+ * holds [q_heads | kv_heads | kv_heads] x head_dim: q is rotated and rounded
+ * once into q_out [rows, q_heads, head_dim] (x_dtype; NULL when q_heads is 0),
+ * k is rotated and v taken as it is, both in fp32, and stored as codes.
+ * cos/sin are [positions, rotary_dim/2] fp32 tables (rotary_dim a multiple of
+ * 16, at most head_dim; 0 = no rotation), rotating pairs (2i, 2i+1)
+ * (interleaved = 1) or (i, i + rotary_dim/2) of the first rotary_dim elements.
+ * A row whose position has no table row is not appended and its q is NaN.
+ *
+ * Page scale: with `old` tokens in the page before the call and amax the
+ * largest magnitude that it gains (NaN left out, infinities as the largest
+ * finite scale), scale' = max(amax * fl(1/127), 2^-120, old ? scale : 0).
+ * Held tokens become round(code * (scale / scale')) and new ones
+ * round(x / scale') within [-127, 127] (a NaN becomes zero), both rounded to
+ * even, so a page's codes do not depend on the order of the work. */
+int tq_paged_append(const tq_paged_kv* kv, const tq_paged_batch* batch, const void* qkv, int x_dtype,
+                    int64_t qkv_stride, int q_heads, const float* cos_table, const float* sin_table,
+                    int64_t positions, int rotary_dim, int interleaved, void* q_out, tq_stream_t stream);
+
+/* k_out, v_out [n, kv_heads, page_size, head_dim] (out_dtype, 16-byte aligned):
+ * the values of pages ids[0..n); NaN for an id outside the pool. */
+int tq_paged_dequantize(const tq_paged_kv* kv, const int32_t* ids, int64_t n, void* k_out, void* v_out,
+                        int out_dtype, tq_stream_t stream);
+
+/* Causal grouped-query attention of the batch's rows over the pool (which
+ * already holds them, e.g. by tq_paged_append): row t of sequence s attends
+ * positions [0, base + t] with base = lengths[s] (counted = 0: lengths as they
+ * were before the rows) or lengths[s] - rows of s (counted = 1).  q is
+ * [rows, q_heads, head_dim] (TQ_F16 or TQ_BF16, row stride q_stride elements,
+ * 16-byte aligned); query head h attends kv head h / (q_heads / kv_heads).
+ * out [rows, q_heads, head_dim] (q's type, contiguous) =
+ * softmax(scale * q . K^T) V; a row that attends nothing is 0 with lse -inf.
+ * lse (nullable) [rows, q_heads] fp32 receives the natural-log sum-exp.
+ * Positions whose page is missing are not attended.
+ * max_context bounds the tokens of any sequence, new ones included; it sizes
+ * the launch only.  The workspace needs no initial value. */
+int tq_paged_attend_workspace_size(const tq_paged_kv* kv, int q_heads, int max_new_tokens, size_t* bytes);
+int tq_paged_attend(const tq_paged_kv* kv, const tq_paged_batch* batch, const void* q, int q_dtype, int64_t q_stride,
+                    int q_heads, int counted, float scale, int64_t max_context, void* out, float* lse,
+                    void* workspace, size_t workspace_bytes, tq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

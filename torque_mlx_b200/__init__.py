@@ -59,7 +59,8 @@ from .artifact import (  # noqa: E402
     convert_npz_checkpoint,
     load_torque_artifact,
 )
+from .paged import PagedKV8Cache  # noqa: E402
 from .conversion import FusedAttentionWeights, fuse_attention_weights  # noqa: E402
 
-__all__ += ["FusedAttentionWeights", "TorqueArtifact", "TorqueArtifactManifest", "build_torque_artifact",
+__all__ += ["FusedAttentionWeights", "PagedKV8Cache", "TorqueArtifact", "TorqueArtifactManifest", "build_torque_artifact",
             "convert_npz_checkpoint", "fuse_attention_weights", "load_torque_artifact"]

@@ -77,6 +77,12 @@ SIGNATURES: dict[str, tuple] = {
                            c_void_p]),
     "tq_silu_mul": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_void_p]),
     "tq_gemv": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_float, c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "tq_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int,
+                                c_int, c_void_p, c_void_p]),
+    "tq_paged_dequantize": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]),
+    "tq_paged_attend_workspace_size": (c_int, [c_void_p, c_int, c_int, POINTER(c_size_t)]),
+    "tq_paged_attend": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_float, c_int64, c_void_p,
+                                c_void_p, c_void_p, c_size_t, c_void_p]),
     "tq_lse_merge": (c_int, [c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p, c_int, c_void_p,
                              c_void_p, c_void_p]),
 }
