@@ -426,6 +426,66 @@ int tq_paged_attend(const tq_paged_kv* kv, const tq_paged_batch* batch, const vo
                     int q_heads, int counted, float scale, int64_t max_context, void* out, float* lse,
                     void* workspace, size_t workspace_bytes, tq_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Linear layers with 4-bit weights, for a few tokens.  New in this build (the
+ * reference keeps its weights in 16 bits; no counterpart).
+ *
+ * A weight [n, k] is held as 4-bit codes with a bf16 scale for each row and
+ * group of group_size (32, 64 or 128) columns: w = scale * (code - 8).  Plain
+ * form: packed [n, ceil(k/2)] bytes, column 2i in the low half; scales
+ * [n, ceil(k/group_size)].  The product reads a laid-out form in which a warp's
+ * operand fragment is 512 consecutive bytes; tq_w4_sizes gives its sizes and
+ * tq_w4_layout builds it once.
+ * ------------------------------------------------------------------------- */
+
+#define TQ_W4_MAX_TOKENS 32 /* tokens of one launch; more are taken 32 at a time */
+
+int tq_w4_sizes(int64_t n, int64_t k, int group_size, size_t* code_bytes, size_t* scale_bytes);
+int tq_w4_layout(const uint8_t* packed, const void* scales, int64_t n, int64_t k, int group_size, void* codes_out,
+                 void* scales_out, tq_stream_t stream);
+/* packed and scales of a weight [n, k] (any tq_dtype): scale = bf16(max|w| / 7)
+ * of the group (2^-100 at least), code = round(w / scale) + 8 within [0, 15]. */
+int tq_w4_quantize(const void* weight, int dtype, int64_t n, int64_t k, int group_size, uint8_t* packed,
+                   void* scales, tq_stream_t stream);
+/* out [n, k] (any tq_dtype) = the laid-out weight's values. */
+int tq_w4_dequantize(const void* codes, const void* scales, int64_t n, int64_t k, int group_size, void* out,
+                     int out_dtype, tq_stream_t stream);
+
+/* y[m, i] = round(sum_j w[i, j] x'[m, j] (+ residual[m, i])) for m in
+ * [0, tokens), fp32 accumulation.  x' as in tq_gemv: x_mode 0 x as it is
+ * (x_dtype TQ_BF16 or TQ_F16, which is y's type too), and for TQ_BF16 also
+ * 1 bf16(x) of an fp32 x, 2 tq_rmsnorm(x), 3 tq_silu_mul of [gate | up] rows of
+ * 2k.  x has row stride x_stride elements; y and residual are [tokens, n]
+ * contiguous.  workspace: tq_gemv_w4_workspace_size bytes (0 for most sizes). */
+int tq_gemv_w4_workspace_size(int64_t n, int64_t k, int64_t tokens, size_t* bytes);
+int tq_gemv_w4(const void* codes, const void* scales, int64_t n, int64_t k, int group_size, const void* x,
+               int x_dtype, int64_t x_stride, int x_mode, const void* norm_weight, float eps, const void* residual,
+               void* y, int64_t tokens, void* workspace, size_t workspace_bytes, tq_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Verification of drafted tokens (speculative sampling).  New in this build.
+ *
+ * Sequence b has draft_counts[b] drafts (NULL: `drafts` each; values outside
+ * [0, drafts] are taken to the nearest) tokens[b, i], proposed with the
+ * probabilities draft[b, i, :] where the target has target[b, i, :]
+ * (`drafts` + 1 rows; dtype any tq_dtype, the same for both; strides in
+ * elements, the vocabulary contiguous).  draft NULL: the drafter was certain,
+ * q = 1 at its token.
+ * Draft i is accepted while uniform[b, i] * q_i < p_i (fp32 product) at its
+ * token; accepted[b] = how many.  The next token is the v that maximises
+ * weight_v / noise[b, v] (fp32, lowest v on ties) over positive weights, with
+ * weight = max(p - q, 0) of the rejected step, or p where every draft was
+ * accepted or that is zero everywhere: with unit-exponential noise a draw from
+ * the normalised weights, from given numbers and without a sum.  out_tokens
+ * [b, 0..drafts] receives the accepted drafts, the next token and -1s.  A
+ * token id outside [0, vocab) is rejected; without a positive weight the next
+ * token is 0. */
+int tq_verify_drafts(const void* target, int64_t target_stride_seq, int64_t target_stride_row, const void* draft,
+                     int64_t draft_stride_seq, int64_t draft_stride_row, int dtype, const int32_t* tokens,
+                     const int32_t* draft_counts, const float* uniform, const float* noise, int64_t noise_stride,
+                     int64_t seqs, int drafts, int64_t vocab, int32_t* accepted, int32_t* out_tokens,
+                     tq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

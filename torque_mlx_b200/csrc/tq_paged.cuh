@@ -110,6 +110,10 @@ inline int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t 
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;"); }
 
+// whether fp16 holds the type's values as they are
+template <typename T> struct Exact { static constexpr bool fp16 = false; };
+template <> struct Exact<__half> { static constexpr bool fp16 = true; };
+
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }

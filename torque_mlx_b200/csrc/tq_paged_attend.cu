@@ -171,10 +171,6 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
   return v;
 }
 
-// whether fp16 holds the type's values as they are
-template <typename T> struct Exact { static constexpr bool fp16 = false; };
-template <> struct Exact<__half> { static constexpr bool fp16 = true; };
-
 template <int D> struct AttendShape {
   static constexpr int kTile = kChunk * D;                 // bytes of a chunk's k (or v) codes
   static constexpr int kStage = 2 * kTile;
