@@ -434,7 +434,7 @@ int tq_paged_attend(const tq_paged_kv* kv, const tq_paged_batch* batch, const vo
  * group of group_size (32, 64 or 128) columns: w = scale * (code - 8).  Plain
  * form: packed [n, ceil(k/2)] bytes, column 2i in the low half; scales
  * [n, ceil(k/group_size)].  The product reads a laid-out form in which a warp's
- * operand fragment is 512 consecutive bytes; tq_w4_sizes gives its sizes and
+ * operand fragments are 1024 consecutive bytes; tq_w4_sizes gives its sizes and
  * tq_w4_layout builds it once.
  * ------------------------------------------------------------------------- */
 

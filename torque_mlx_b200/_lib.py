@@ -145,6 +145,14 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def stream_of(index: int) -> int:
+    """Handle of device ``index``'s current CUDA stream."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

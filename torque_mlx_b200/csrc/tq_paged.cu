@@ -12,7 +12,6 @@
 
 namespace tq {
 
-constexpr int kAppendThreads = 128;
 constexpr float kInv127 = 1.0f / 127.0f;
 constexpr float kScaleFloor = 7.52316385e-37f;  // 2^-120: a page of zeros keeps a positive scale
 constexpr float kScaleMost = 3.402823466e38f * kInv127;
@@ -25,46 +24,60 @@ struct RopeArgs {
   int interleaved;
 };
 
-// Item i of a head's row: two vectors of eight elements at e0 and e1, such
-// that rotary pairs lie within an item.  Values come back rotated, with the
-// elementwise roundings of separate products and sums (no contraction), so
+// The rotation of item i of a head's row at one position.  An item is two
+// vectors of eight elements, at e0 and e1, such that rotary pairs lie within
+// it; the same item of every head of the row shares it.  Values come back with
+// the elementwise roundings of separate products and sums (no contraction), so
 // that they equal the same formula written with single fp32 operations.
+struct ItemRope {
+  float c[8], s[8];
+  int e0, e1;
+  bool live, interleaved;
+
+  __device__ __forceinline__ ItemRope(const RopeArgs& r, int i, bool rotate, int64_t pos) {
+    live = rotate && i * 16 < r.dim;
+    interleaved = r.interleaved;
+    e0 = 16 * i;
+    e1 = e0 + 8;
+    if (!live) return;
+    if (!interleaved) {
+      e0 = 8 * i;
+      e1 = r.dim / 2 + 8 * i;
+    }
+    load8(r.cos + pos * (r.dim / 2) + 8 * i, c);
+    load8(r.sin + pos * (r.dim / 2) + 8 * i, s);
+  }
+  __device__ __forceinline__ void apply(float (&a)[8], float (&b)[8]) const {
+    if (!live) return;
+    if (interleaved) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = a[2 * j], y = a[2 * j + 1], u = b[2 * j], v = b[2 * j + 1];
+        a[2 * j] = __fsub_rn(__fmul_rn(x, c[j]), __fmul_rn(y, s[j]));
+        a[2 * j + 1] = __fadd_rn(__fmul_rn(x, s[j]), __fmul_rn(y, c[j]));
+        b[2 * j] = __fsub_rn(__fmul_rn(u, c[4 + j]), __fmul_rn(v, s[4 + j]));
+        b[2 * j + 1] = __fadd_rn(__fmul_rn(u, s[4 + j]), __fmul_rn(v, c[4 + j]));
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = a[j], y = b[j];
+        a[j] = __fsub_rn(__fmul_rn(x, c[j]), __fmul_rn(y, s[j]));
+        b[j] = __fadd_rn(__fmul_rn(x, s[j]), __fmul_rn(y, c[j]));
+      }
+    }
+  }
+};
+
 template <typename T>
 __device__ __forceinline__ void load_item(const T* head, int i, const RopeArgs& r, bool rotate, int64_t pos,
                                           float (&a)[8], float (&b)[8], int& e0, int& e1) {
-  const bool live = rotate && i * 16 < r.dim;
-  if (live && !r.interleaved) {
-    e0 = 8 * i;
-    e1 = r.dim / 2 + 8 * i;
-  } else {
-    e0 = 16 * i;
-    e1 = e0 + 8;
-  }
+  const ItemRope rope(r, i, rotate, pos);
+  e0 = rope.e0;
+  e1 = rope.e1;
   load8(head + e0, a);
   load8(head + e1, b);
-  if (!live) return;
-  const float4* c4 = reinterpret_cast<const float4*>(r.cos + pos * (r.dim / 2) + 8 * i);
-  const float4* s4 = reinterpret_cast<const float4*>(r.sin + pos * (r.dim / 2) + 8 * i);
-  const float4 c0 = __ldg(c4), c1 = __ldg(c4 + 1), s0 = __ldg(s4), s1 = __ldg(s4 + 1);
-  const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-  const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-  if (r.interleaved) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x = a[2 * j], y = a[2 * j + 1], u = b[2 * j], v = b[2 * j + 1];
-      a[2 * j] = __fsub_rn(__fmul_rn(x, c[j]), __fmul_rn(y, s[j]));
-      a[2 * j + 1] = __fadd_rn(__fmul_rn(x, s[j]), __fmul_rn(y, c[j]));
-      b[2 * j] = __fsub_rn(__fmul_rn(u, c[4 + j]), __fmul_rn(v, s[4 + j]));
-      b[2 * j + 1] = __fadd_rn(__fmul_rn(u, s[4 + j]), __fmul_rn(v, c[4 + j]));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = a[j], y = b[j];
-      a[j] = __fsub_rn(__fmul_rn(x, c[j]), __fmul_rn(y, s[j]));
-      b[j] = __fadd_rn(__fmul_rn(x, s[j]), __fmul_rn(y, c[j]));
-    }
-  }
+  rope.apply(a, b);
 }
 
 // Biased code of x: a NaN becomes zero (the conversion gives 0 for it).
@@ -72,70 +85,117 @@ __device__ __forceinline__ uint32_t code_of(float x) {
   return (uint32_t)(min(127, max(-127, __float2int_rn(x))) + 128);
 }
 
-__device__ __forceinline__ uint2 codes8(const float (&x)[8], float scale) {
+// Biased codes of round(x / scale).  The product with 1 / scale is within 2e-5
+// of the quotient (127 of it, three roundings of 2^-24), so its nearest whole
+// number is the quotient's unless it lies within 1e-4 of a half; then the
+// quotient itself decides.  Adding 1.5 * 2^23 + 128 rounds to even and leaves
+// the biased code in the low byte.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float scale, float inv) {
+  constexpr float kMagic = 12582912.f + 128.f;
   uint32_t w[2] = {0, 0};
+  bool near = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i / 4] |= code_of(__fdiv_rn(x[i], scale)) << (8 * (i & 3));
+  for (int i = 0; i < 8; ++i) {
+    float y = __fmul_rn(x[i], inv);
+    y = y == y ? fminf(fmaxf(y, -127.f), 127.f) : 0.f;
+    const float m = __fadd_rn(y, kMagic);
+    near |= fabsf(__fsub_rn(y, __fsub_rn(m, kMagic))) > 0.4999f;
+    w[i / 4] |= (__float_as_uint(m) & 255u) << (8 * (i & 3));
+  }
+  if (near) {
+    w[0] = w[1] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i / 4] |= code_of(__fdiv_rn(x[i], scale)) << (8 * (i & 3));
+  }
   return make_uint2(w[0], w[1]);
 }
 
-// grid (seqs * pages, kv_heads, 3): z = 0 the k codes of a page and head, 1
-// its v codes, 2 the q heads of that kv head for the page's tokens.
-template <typename T>
-__global__ void __launch_bounds__(kAppendThreads)
+// grid (seqs * pages, kv_heads, 2 + q parts): z = 0 the k codes of a page and
+// head, 1 its v codes, from 2 on q_each of that kv head's q heads for the
+// page's tokens.
+//
+// A thread keeps the values of its first kHold items from the first pass to
+// the second in registers, which covers pages of 64 x 128; longer ones read
+// the rest of their rows again.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS)
 paged_append_kernel(const tq_paged_kv kv, const tq_paged_batch bt, const T* __restrict__ qkv, int64_t stride, int q_heads,
-                    const RopeArgs rope, T* __restrict__ q_out, int pages) {
-  __shared__ float red[kAppendThreads / 32];
+                    int q_each, const RopeArgs rope, T* __restrict__ q_out, int pages) {
+  constexpr int kHold = THREADS == 128 ? 1 : 2;
+  __shared__ float red[THREADS / 32];
   grid_wait();
   const int s = blockIdx.x / pages, j = blockIdx.x - s * pages;
-  const int h = blockIdx.y, d = kv.head_dim, P = kv.page_size, items = d / 16;
+  const int h = blockIdx.y, d = kv.head_dim, P = kv.page_size;
+  const int shift = d == 64 ? 2 : d == 128 ? 3 : 4, items = 1 << shift;  // items of a head's row
   const RowSpan span = row_span(bt, s);
   const int first_page = span.len / P;
   const int page = first_page + j;
   const int64_t p0 = (int64_t)page * P;                     // first position of the page
   const int lo = j == 0 ? span.len - (int)p0 : 0;           // first slot written
-  int hi = (int)min((int64_t)P, (int64_t)span.len + span.n - p0);  // past the last one
+  const int hi = (int)min((int64_t)P, (int64_t)span.len + span.n - p0);  // past the last one
   if (span.n == 0 || hi <= lo) return;
   const int64_t row0 = span.first + (p0 + lo - span.len);   // row of slot lo
   const int tid = threadIdx.x;
   int64_t known = hi - lo;                                  // tokens whose position has a rotary row
   if (rope.dim) known = min(known, max((int64_t)0, rope.positions - (p0 + lo)));
 
-  if (blockIdx.z == 2) {
-    const int group = q_heads / kv.kv_heads, per_row = group * items;
-    const int total = (hi - lo) * per_row;
-    for (int it = tid; it < total; it += kAppendThreads) {
-      const int t = it / per_row, rest = it - t * per_row;
-      const int head = h * group + rest / items, i = rest % items;
-      float a[8], b[8];
-      int e0, e1;
-      load_item(qkv + (row0 + t) * stride + (int64_t)head * d, i, rope, t < known, p0 + lo + t, a, b, e0, e1);
-      if (t >= known) {
+  if (blockIdx.z >= 2) {
+    const int group = q_heads / kv.kv_heads, g0 = (blockIdx.z - 2) * q_each, g1 = min(group, g0 + q_each);
+    const int total = (hi - lo) * items;
+    for (int it = tid; it < total; it += THREADS) {
+      const int t = it >> shift, i = it & (items - 1);
+      const ItemRope r(rope, i, t < known, p0 + lo + t);
+      const T* x = qkv + (row0 + t) * stride + (int64_t)(h * group) * d;
+      T* o = q_out + ((row0 + t) * (int64_t)q_heads + h * group) * d;
+#pragma unroll 4
+      for (int g = g0; g < g1; ++g) {
+        float a[8], b[8];
+        load8(x + g * d + r.e0, a);
+        load8(x + g * d + r.e1, b);
+        r.apply(a, b);
+        if (t >= known) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) a[k] = b[k] = __int_as_float(0x7fffffff);
+          for (int k = 0; k < 8; ++k) a[k] = b[k] = __int_as_float(0x7fffffff);
+        }
+        store8(o + g * d + r.e0, a);
+        store8(o + g * d + r.e1, b);
       }
-      T* o = q_out + (row0 + t) * (int64_t)q_heads * d + (int64_t)head * d;
-      store8(o + e0, a);
-      store8(o + e1, b);
     }
     return;
   }
 
   const bool is_v = blockIdx.z == 1;
-  const int id = page_id(kv, bt, s, page);
   const int n = (int)known;
-  if (id < 0 || n <= 0) return;
+  if (n <= 0) return;
   const T* src = qkv + row0 * stride + (int64_t)(q_heads + (is_v ? kv.kv_heads : 0) + h) * d;
+  const int total = n * items;
+  float top = 0.f;
+  float va[kHold][8], vb[kHold][8];
+  int e0[kHold], e1[kHold];
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) {
+    const int it = tid + u * THREADS;
+    if (it < total) {
+      const int t = it >> shift, i = it & (items - 1);
+      load_item(src + t * stride, i, rope, !is_v, p0 + lo + t, va[u], vb[u], e0[u], e1[u]);
+    }
+  }
+  const int id = page_id(kv, bt, s, page);
+  if (id < 0) return;
   uint8_t* codes = (is_v ? kv.v_pages : kv.k_pages) + ((int64_t)id * kv.kv_heads + h) * P * d;
   float* scale_at = (is_v ? kv.v_scales : kv.k_scales) + (int64_t)id * kv.kv_heads + h;
   const float was = lo > 0 ? *scale_at : 0.f;
-
-  float top = 0.f;
-  for (int it = tid; it < n * items; it += kAppendThreads) {
-    const int t = it / items, i = it - t * items;
+#pragma unroll
+  for (int u = 0; u < kHold; ++u)
+    if (tid + u * THREADS < total) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, fmaxf(fabsf(va[u][k]), fabsf(vb[u][k])));
+    }
+  for (int it = tid + kHold * THREADS; it < total; it += THREADS) {
+    const int t = it >> shift, i = it & (items - 1);
     float a[8], b[8];
-    int e0, e1;
-    load_item(src + t * stride, i, rope, !is_v, p0 + lo + t, a, b, e0, e1);
+    int x0, x1;
+    load_item(src + t * stride, i, rope, !is_v, p0 + lo + t, a, b, x0, x1);
 #pragma unroll
     for (int k = 0; k < 8; ++k) top = fmaxf(top, fmaxf(fabsf(a[k]), fabsf(b[k])));
   }
@@ -144,15 +204,16 @@ paged_append_kernel(const tq_paged_kv kv, const tq_paged_batch bt, const T* __re
   if ((tid & 31) == 0) red[tid >> 5] = top;
   __syncthreads();  // also: every thread has read the old scale
 #pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) top = fmaxf(top, red[w]);
+  for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, red[w]);
   float scale = fminf(fmaxf(__fmul_rn(top, kInv127), kScaleFloor), kScaleMost);
   if (lo > 0) scale = fmaxf(scale, was);
   if (tid == 0) *scale_at = scale;
+  const float inv = __fdiv_rn(1.f, scale);
 
   if (lo > 0 && scale != was) {  // the tokens held move to the larger scale
     const float ratio = __fdiv_rn(was, scale);
     uint4* p = reinterpret_cast<uint4*>(codes);
-    for (int i = tid; i < lo * items; i += kAppendThreads) {
+    for (int i = tid; i < lo * items; i += THREADS) {
       uint4 v = p[i];
       uint32_t* w = &v.x;
 #pragma unroll
@@ -166,14 +227,23 @@ paged_append_kernel(const tq_paged_kv kv, const tq_paged_batch bt, const T* __re
       p[i] = v;
     }
   }
-  for (int it = tid; it < n * items; it += kAppendThreads) {
-    const int t = it / items, i = it - t * items;
+#pragma unroll
+  for (int u = 0; u < kHold; ++u) {
+    const int it = tid + u * THREADS;
+    if (it < total) {
+      uint8_t* o = codes + (int64_t)(lo + (it >> shift)) * d;
+      *reinterpret_cast<uint2*>(o + e0[u]) = codes8(va[u], scale, inv);
+      *reinterpret_cast<uint2*>(o + e1[u]) = codes8(vb[u], scale, inv);
+    }
+  }
+  for (int it = tid + kHold * THREADS; it < total; it += THREADS) {
+    const int t = it >> shift, i = it & (items - 1);
     float a[8], b[8];
-    int e0, e1;
-    load_item(src + t * stride, i, rope, !is_v, p0 + lo + t, a, b, e0, e1);
+    int x0, x1;
+    load_item(src + t * stride, i, rope, !is_v, p0 + lo + t, a, b, x0, x1);
     uint8_t* o = codes + (int64_t)(lo + t) * d;
-    *reinterpret_cast<uint2*>(o + e0) = codes8(a, scale);
-    *reinterpret_cast<uint2*>(o + e1) = codes8(b, scale);
+    *reinterpret_cast<uint2*>(o + x0) = codes8(a, scale, inv);
+    *reinterpret_cast<uint2*>(o + x1) = codes8(b, scale, inv);
   }
 }
 
@@ -214,9 +284,23 @@ int launch_append(const tq_paged_kv& kv, const tq_paged_batch& b, const void* qk
   const int pages = (b.max_new_tokens + kv.page_size - 2) / kv.page_size + 1;
   const int64_t x = (int64_t)b.seqs * pages;
   if (x > INT32_MAX || kv.kv_heads > 65535) return TQ_E_SHAPE;
-  return launch_dependent(paged_append_kernel<T>, dim3((unsigned)x, kv.kv_heads, q_heads ? 3 : 2),
-                          dim3(kAppendThreads), 0, stream, kv, b, (const T*)qkv, stride, q_heads, rope, (T*)q_out,
-                          pages);
+  // 128 threads while a page gains few tokens, 256 for prompts; the q heads of
+  // a kv head share a CTA (and the angles a thread loads) up to eight rows of
+  // items a thread.
+  const int rows = b.max_new_tokens < kv.page_size ? b.max_new_tokens : kv.page_size, items = rows * (kv.head_dim / 16);
+  const int group = q_heads / kv.kv_heads;
+  const bool wide = items > 128;
+  const int threads = wide ? 256 : 128;
+  int each = 16 * threads / items;
+  each = each < 1 ? 1 : (each > group ? group : each);
+  const int parts = group ? (group + each - 1) / each : 0;
+  if (parts > 65533) return TQ_E_SHAPE;
+  const dim3 grid((unsigned)x, kv.kv_heads, 2 + parts);
+  if (wide)
+    return launch_dependent(paged_append_kernel<T, 256>, grid, dim3(256), 0, stream, kv, b, (const T*)qkv, stride,
+                            q_heads, each, rope, (T*)q_out, pages);
+  return launch_dependent(paged_append_kernel<T, 128>, grid, dim3(128), 0, stream, kv, b, (const T*)qkv, stride, q_heads,
+                          each, rope, (T*)q_out, pages);
 }
 
 }  // namespace tq

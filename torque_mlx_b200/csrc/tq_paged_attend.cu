@@ -31,6 +31,7 @@ constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = kAttendWarps * 32;
 constexpr int kChunk = 16;    // tokens of a ring stage
 constexpr int kMinChunks = 8; // smallest share of a CTA
+constexpr int kWholeChunks = 32;
 constexpr float kNoScore = -1e30f;  // finite, so that differences of two of them are not NaN
 constexpr float kLazy = 8.f;  // a score may pass its reference by 2^8 before the sums are rescaled
 
@@ -47,6 +48,7 @@ struct AttendArgs {
   int group;
   int counted;
   int ctas;
+  int whole;       // units are not divided
   float scale2;    // softmax scale times log2(e)
 };
 
@@ -55,6 +57,7 @@ struct SeqWork {
   int n, base;    // rows; position of the first one
   int tiles;      // query tiles of a kv head
   int chunks;     // chunks of a unit
+  int weight;     // its length on the line: its chunks, or 1 where units are not divided
 };
 
 template <int ROWS>
@@ -69,6 +72,7 @@ __device__ __forceinline__ SeqWork seq_work(const AttendArgs& a, int s) {
   w.base = a.counted ? held - r.n : held;
   w.tiles = (int)(((int64_t)r.n * a.group + ROWS - 1) / ROWS);
   w.chunks = max(1, (w.base + r.n + kChunk - 1) / kChunk);
+  w.weight = a.whole ? 1 : w.chunks;
   return w;
 }
 
@@ -83,7 +87,7 @@ __device__ __forceinline__ void plan_prefix(const AttendArgs& a, int64_t* prefix
     int64_t w = 0;
     if (s < a.bt.seqs) {
       const SeqWork q = seq_work<ROWS>(a, s);
-      w = (int64_t)q.tiles * a.kv.kv_heads * q.chunks;
+      w = (int64_t)q.tiles * a.kv.kv_heads * q.weight;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -104,8 +108,8 @@ __device__ __forceinline__ void plan_prefix(const AttendArgs& a, int64_t* prefix
   __syncthreads();
 }
 
-__device__ __forceinline__ int64_t used_ctas(int64_t total, int ctas) {
-  const int64_t most = (total + kMinChunks - 1) / kMinChunks;
+__device__ __forceinline__ int64_t used_ctas(const AttendArgs& a, int64_t total) {
+  const int64_t ctas = a.ctas, most = a.whole ? total : (total + kMinChunks - 1) / kMinChunks;
   return most < 1 ? 1 : (most < ctas ? most : ctas);
 }
 
@@ -174,7 +178,7 @@ __device__ __forceinline__ uint2 lds64(uint32_t at) {
 template <int D> struct AttendShape {
   static constexpr int kTile = kChunk * D;                 // bytes of a chunk's k (or v) codes
   static constexpr int kStage = 2 * kTile;
-  static constexpr int kStages = D == 64 ? 6 : 3;
+  static constexpr int kStages = D == 64 ? 6 : (D == 128 ? 3 : 2);
   static constexpr int kPieces = D / 16;                   // 16-byte pieces of a token
   // Piece p of token t lies at piece p ^ swizzle(t): the eight lanes that the
   // shared memory serves together then meet eight different 16-byte columns,
@@ -198,7 +202,7 @@ paged_attend_kernel(const AttendArgs a) {
   plan_prefix<ROWS, kAttendThreads>(a, prefix);
   grid_trigger();
   const int64_t total = prefix[a.bt.seqs];
-  const int64_t ctas = used_ctas(total, a.ctas);
+  const int64_t ctas = used_ctas(a, total);
   if ((int64_t)blockIdx.x >= ctas) return;
   int64_t pos = (int64_t)blockIdx.x * total / ctas;
   const int64_t end = ((int64_t)blockIdx.x + 1) * total / ctas;
@@ -211,13 +215,55 @@ paged_attend_kernel(const AttendArgs a) {
     const int s = find_seq(prefix, a.bt.seqs, pos);
     const SeqWork w = seq_work<ROWS>(a, s);
     const int64_t rel = pos - prefix[s];
-    const int unit = (int)(rel / w.chunks), c0 = (int)(rel - (int64_t)unit * w.chunks);
-    const int c1 = (int)min((int64_t)w.chunks, c0 + (end - pos));
+    const int unit = (int)(rel / w.weight), c0 = (int)(rel - (int64_t)unit * w.weight);
+    const int c1 = a.whole ? w.chunks : (int)min((int64_t)w.chunks, c0 + (end - pos));
     const int h = unit / w.tiles, r0 = (unit - h * w.tiles) * ROWS;
     const int nr = min(ROWS, w.n * a.group - r0);             // rows of this tile
     const int last = w.base + (r0 + nr - 1) / a.group;        // last position that any of them attends
     const int free_to = w.base + r0 / a.group;                // positions up to here need no mask
-    pos += c1 - c0;
+    pos += a.whole ? 1 : c1 - c0;
+
+    // ---- the warp's chunks: c0 + warp, c0 + warp + 4, ... ----
+    const int steps = min(c1, last / kChunk + 1) > c0 + warp && last >= 0
+                          ? (min(c1, last / kChunk + 1) - c0 - warp + kAttendWarps - 1) / kAttendWarps
+                          : 0;
+    auto chunk_page = [&](int it) {
+      const int ch = c0 + warp + it * kAttendWarps;
+      return it < steps ? page_id(a.kv, a.bt, s, ch * kChunk / P) : -1;
+    };
+    int ids = chunk_page(lane), ids_next = chunk_page(32 + lane);
+    int issued = 0;
+    auto issue = [&](int st) {  // copies of step `issued` into ring stage st
+      if (issued < steps) {
+        const int id = __shfl_sync(FULL, ids, issued & 31);
+        if (id >= 0) {
+          const int ch = c0 + warp + issued * kAttendWarps;
+          const int64_t block = (int64_t)id * Hkv + h;
+          const int64_t at = (block * P + (ch * kChunk) % P) * D;
+          const uint8_t* ks = a.kv.k_pages + at + lane * 16;
+          const uint8_t* vs = a.kv.v_pages + at + lane * 16;
+          const uint32_t dst = ring_at + st * Shape::kStage;
+#pragma unroll
+          for (int i = 0; i < kChunk * D / 512; ++i) {
+            const int piece = lane + 32 * i, t = piece / Shape::kPieces, p = piece % Shape::kPieces;
+            const uint32_t off = t * D + ((p ^ Shape::swizzle(t)) << 4);
+            cp_async16(dst + off, ks + 512 * i);
+            cp_async16(dst + Shape::kTile + off, vs + 512 * i);
+          }
+          if (lane < 2) cp_async4(head_at + (st * 2 + lane) * 4, (lane ? a.kv.v_scales : a.kv.k_scales) + block);
+        } else if (lane == 0) {
+          head[warp][st][0] = -1.f;  // no page: the chunk is not attended
+        }
+        ++issued;
+        if ((issued & 31) == 0) {
+          ids = ids_next;
+          ids_next = chunk_page(issued + 32 + lane);
+        }
+      }
+      cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i);
 
     // ---- query rows: B fragments of k = (piece, word) steps, exact in fp16 ----
     uint32_t qb[NT][KI * 4][2];
@@ -280,48 +326,6 @@ paged_attend_kernel(const AttendArgs a) {
         for (int k = 0; k < 4; ++k) o[mt][nt][k] = 0.f;
     }
 
-    // ---- the warp's chunks: c0 + warp, c0 + warp + 4, ... ----
-    const int steps = min(c1, last / kChunk + 1) > c0 + warp && last >= 0
-                          ? (min(c1, last / kChunk + 1) - c0 - warp + kAttendWarps - 1) / kAttendWarps
-                          : 0;
-    auto chunk_page = [&](int it) {
-      const int ch = c0 + warp + it * kAttendWarps;
-      return it < steps ? page_id(a.kv, a.bt, s, ch * kChunk / P) : -1;
-    };
-    int ids = chunk_page(lane), ids_next = chunk_page(32 + lane);
-    int issued = 0;
-    auto issue = [&](int st) {  // copies of step `issued` into ring stage st
-      if (issued < steps) {
-        const int id = __shfl_sync(FULL, ids, issued & 31);
-        if (id >= 0) {
-          const int ch = c0 + warp + issued * kAttendWarps;
-          const int64_t block = (int64_t)id * Hkv + h;
-          const int64_t at = (block * P + (ch * kChunk) % P) * D;
-          const uint8_t* ks = a.kv.k_pages + at + lane * 16;
-          const uint8_t* vs = a.kv.v_pages + at + lane * 16;
-          const uint32_t dst = ring_at + st * Shape::kStage;
-#pragma unroll
-          for (int i = 0; i < kChunk * D / 512; ++i) {
-            const int piece = lane + 32 * i, t = piece / Shape::kPieces, p = piece % Shape::kPieces;
-            const uint32_t off = t * D + ((p ^ Shape::swizzle(t)) << 4);
-            cp_async16(dst + off, ks + 512 * i);
-            cp_async16(dst + Shape::kTile + off, vs + 512 * i);
-          }
-          if (lane < 2) cp_async4(head_at + (st * 2 + lane) * 4, (lane ? a.kv.v_scales : a.kv.k_scales) + block);
-        } else if (lane == 0) {
-          head[warp][st][0] = -1.f;  // no page: the chunk is not attended
-        }
-        ++issued;
-        if ((issued & 31) == 0) {
-          ids = ids_next;
-          ids_next = chunk_page(issued + 32 + lane);
-        }
-      }
-      cp_commit();
-    };
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(i);
-
     int st = 0;
     for (int it = 0; it < steps; ++it, st = st + 1 == STAGES ? 0 : st + 1) {
       cp_wait<STAGES - 2>();
@@ -334,11 +338,14 @@ paged_attend_kernel(const AttendArgs a) {
       const uint32_t kt = ring_at + st * Shape::kStage, vt = kt + Shape::kTile;
 
       // scores of tokens g, g + 8 with rows 2c, 2c + 1
-      float sc[NT][4];
+      constexpr int CHAINS = D == 256 ? 2 : 1;  // sums that run side by side
+      float sums[CHAINS][NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int x = 0; x < CHAINS; ++x)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sc[nt][k] = 0.f;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sums[x][nt][k] = 0.f;
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
         const int piece = D == 64 ? c : 8 * (i >> 1) + 2 * c + (i & 1);
@@ -350,15 +357,17 @@ paged_attend_kernel(const AttendArgs a) {
           const uint32_t a0 = unbias(prmt(lo[k], 0x64646464u, 0x4140)), a2 = unbias(prmt(lo[k], 0x64646464u, 0x4342));
           const uint32_t a1 = unbias(prmt(hi[k], 0x64646464u, 0x4140)), a3 = unbias(prmt(hi[k], 0x64646464u, 0x4342));
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma16816(sc[nt], a0, a1, a2, a3, qb[nt][i * 4 + k][0], qb[nt][i * 4 + k][1]);
+          for (int nt = 0; nt < NT; ++nt) 
+            mma16816(sums[i % CHAINS][nt], a0, a1, a2, a3, qb[nt][i * 4 + k][0], qb[nt][i * 4 + k][1]);
         }
       }
       bool grow = false;
+      float sc[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          float v = sc[nt][k] * (ks * kf[nt][k & 1]);
+          float v = (CHAINS == 1 ? sums[0][nt][k] : sums[0][nt][k] + sums[CHAINS - 1][nt][k]) * (ks * kf[nt][k & 1]);
           if (tok + kChunk - 1 > free_to && tok + g + 8 * (k >> 1) > limit[nt][k & 1]) v = -INFINITY;
           sc[nt][k] = v;
           grow |= v > m[nt][k & 1] + kLazy || v + lv > m2[nt][k & 1] + kLazy;
@@ -493,48 +502,67 @@ paged_attend_kernel(const AttendArgs a) {
   }
 }
 
-// grid (seqs * kv_heads * tiles, rows): joins the parts of one query row.
-constexpr int kJoinThreads = 256;
+// grid (seqs * kv_heads * tiles, rows, d / DIMS): joins the parts of DIMS
+// elements of one query row.  Few units have many parts each: 256 threads read
+// sixteen of them side by side, 64 elements a CTA.  Many units have two or
+// three: a CTA of 64 threads for a row.
 constexpr int kMaxCtas = 148 * 8;
 
-template <int D, int ROWS, typename T>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendArgs a, int tiles) {
+template <int D, int ROWS, int DIMS, int THREADS, typename T>
+__global__ void __launch_bounds__(THREADS) paged_join_kernel(const AttendArgs a, int tiles) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float weight[kMaxCtas];
-  __shared__ float red[2][kJoinThreads / 32];
-  __shared__ float4 acc[kJoinThreads];
+  __shared__ float red[2][THREADS / 32];
+  __shared__ float4 acc[THREADS];
   int64_t* prefix = reinterpret_cast<int64_t*>(smem);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int tile = blockIdx.x % tiles, h = (blockIdx.x / tiles) % a.kv.kv_heads, s = blockIdx.x / tiles / a.kv.kv_heads;
   const int r = blockIdx.y;
-  // lengths are the step's inputs, which no kernel of the step writes; the
-  // partial outputs are read only after the wait
-  grid_wait();
+  // The attention's CTAs start this kernel after their own wait, so what came
+  // before them (the lengths among it) is complete; their parts are read after
+  // the wait here, which every CTA makes.
   const SeqWork w = seq_work<ROWS>(a, s);
-  if (tile >= w.tiles || tile * ROWS + r >= w.n * a.group) return;
-  plan_prefix<ROWS, kJoinThreads>(a, prefix);
-  const int64_t total = prefix[a.bt.seqs], ctas = used_ctas(total, a.ctas);
-  const int64_t u0 = prefix[s] + ((int64_t)h * w.tiles + tile) * w.chunks;
-  const int first = (int)(((u0 + 1) * ctas - 1) / total), last = (int)(((u0 + w.chunks) * ctas - 1) / total);
+  const bool live = tile < w.tiles && tile * ROWS + r < w.n * a.group;
+  int64_t total = 1, ctas = 1, u0 = 0;
+  if (live) {
+    plan_prefix<ROWS, THREADS>(a, prefix);
+    total = prefix[a.bt.seqs];
+    ctas = used_ctas(a, total);
+    u0 = prefix[s] + ((int64_t)h * w.tiles + tile) * w.weight;
+  }
+  grid_wait();
+  if (!live) return;
+  const int first = (int)(((u0 + 1) * ctas - 1) / total), last = (int)(((u0 + w.weight) * ctas - 1) / total);
   if (first == last) return;  // finished by its CTA
   const int n = last - first + 1;
   const int slot0 = (int64_t)first * total / ctas < u0 ? 1 : 0;
   auto part_of = [&](int i) { return ((int64_t)(first + i) * 2 + (i == 0 ? slot0 : 0)) * ROWS + r; };
+
+  constexpr int Q = DIMS / 4, STEP = THREADS / Q;  // threads of a part; parts side by side
+  const int q = tid % Q, d0 = blockIdx.z * DIMS + 4 * q;
   float top = -INFINITY;
-  for (int i = tid; i < n; i += kJoinThreads) {
+  for (int i = tid; i < n; i += THREADS) {
     const float v = a.part_l[part_of(i)];
     weight[i] = v;
     top = fmaxf(top, v);
+  }
+  // the first parts are on their way while the weights are formed
+  constexpr int AHEAD = 8;
+  float4 x[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = tid / Q + k * STEP;
+    if (i < n) x[k] = *reinterpret_cast<const float4*>(a.part_o + part_of(i) * D + d0);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
   if (lane == 0) red[0][warp] = top;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) top = fmaxf(top, red[0][i]);
+  for (int i = 0; i < THREADS / 32; ++i) top = fmaxf(top, red[0][i]);
   if (top == -INFINITY) top = 0.f;
   float sum = 0.f;
-  for (int i = tid; i < n; i += kJoinThreads) {
+  for (int i = tid; i < n; i += THREADS) {
     const float v = ex2(weight[i] - top);
     weight[i] = v;
     sum += v;
@@ -545,31 +573,34 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const AttendAr
   __syncthreads();
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) sum += red[1][i];
+  for (int i = 0; i < THREADS / 32; ++i) sum += red[1][i];
 
-  constexpr int Q = D / 4, STEP = kJoinThreads / Q;  // threads of a part; parts in flight
-  const int q = tid % Q;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int i = tid / Q; i < n; i += STEP) {
-    const float4 x = reinterpret_cast<const float4*>(a.part_o + part_of(i) * D)[q];
+  auto add = [&](int i, const float4& y) {
     const float f = weight[i];
-    v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
-  }
+    v.x = fmaf(f, y.x, v.x), v.y = fmaf(f, y.y, v.y), v.z = fmaf(f, y.z, v.z), v.w = fmaf(f, y.w, v.w);
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (tid / Q + k * STEP < n) add(tid / Q + k * STEP, x[k]);
+#pragma unroll 8
+  for (int i = tid / Q + AHEAD * STEP; i < n; i += STEP)
+    add(i, *reinterpret_cast<const float4*>(a.part_o + part_of(i) * D + d0));
   acc[tid] = v;
   __syncthreads();
   if (tid < Q) {
 #pragma unroll
     for (int i = 1; i < STEP; ++i) {
-      const float4 x = acc[tid + i * Q];
-      v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      const float4 y = acc[tid + i * Q];
+      v.x += y.x, v.y += y.y, v.z += y.z, v.w += y.w;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int rr = tile * ROWS + r;
     const int64_t row = w.first + rr / a.group, hq = h * a.group + rr % a.group;
-    T* o = reinterpret_cast<T*>(a.out) + (row * a.q_heads + hq) * D + 4 * q;
+    T* o = reinterpret_cast<T*>(a.out) + (row * a.q_heads + hq) * D + d0;
     o[0] = from_f32<T>(v.x * inv), o[1] = from_f32<T>(v.y * inv), o[2] = from_f32<T>(v.z * inv), o[3] = from_f32<T>(v.w * inv);
-    if (a.lse && tid == 0) a.lse[row * a.q_heads + hq] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.69314718f;
+    if (a.lse && tid == 0 && blockIdx.z == 0)
+      a.lse[row * a.q_heads + hq] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.69314718f;
   }
 }
 
@@ -601,11 +632,19 @@ int launch_attend(AttendArgs a, int64_t max_context, cudaStream_t stream) {
   const int64_t units = (int64_t)a.bt.seqs * a.kv.kv_heads * tiles;
   if (units > INT32_MAX) return TQ_E_SHAPE;
   const int64_t chunks = (max_context + kChunk - 1) / kChunk;
-  const int64_t most = units * (chunks < 1 ? 1 : chunks) / kMinChunks + 1;
+  // Units of a few hundred tokens are not divided: the parts' launch would cost
+  // more than the eight steps of a warp that it saves.
+  a.whole = chunks <= kWholeChunks;
+  const int64_t most = a.whole ? units : units * chunks / kMinChunks + 1;
   if (most < a.ctas) a.ctas = (int)most;
   int st = launch_dependent(paged_attend_kernel<D, NT, T>, dim3(a.ctas), dim3(kAttendThreads), smem, stream, a);
-  if (st != TQ_OK || a.ctas == 1) return st;
-  return launch_dependent(paged_join_kernel<D, 8 * NT, T>, dim3((unsigned)units, 8 * NT), dim3(kJoinThreads),
+  if (st != TQ_OK || a.ctas == 1 || a.whole) return st;
+  const int64_t rows = (int64_t)a.bt.max_new_tokens * a.group;
+  const unsigned y = (unsigned)(rows < 8 * NT ? rows : 8 * NT);
+  if (units * 4 >= a.ctas)
+    return launch_dependent(paged_join_kernel<D, 8 * NT, D, 64, T>, dim3((unsigned)units, y), dim3(64), prefix_bytes,
+                            stream, a, tiles);
+  return launch_dependent(paged_join_kernel<D, 8 * NT, 64, 256, T>, dim3((unsigned)units, y, D / 64), dim3(256),
                           prefix_bytes, stream, a, tiles);
 }
 

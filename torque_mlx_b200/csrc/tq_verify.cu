@@ -16,7 +16,7 @@
 
 namespace tq {
 
-constexpr int kVerifyThreads = 512;
+constexpr int kVerifyMostThreads = 512;
 constexpr int kVerifyMostCluster = 16;
 
 struct VerifyArgs {
@@ -45,40 +45,87 @@ __device__ __forceinline__ uint64_t key_of(float weight, float noise, int64_t v)
 
 __device__ __forceinline__ uint64_t best_of(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
+// A thread's best key so far, with a bound that spares most divisions: only a
+// weight above least = (best score, less 2^-20 of it) times its noise can have
+// a score as large as the best (the product and the quotient are off by 2^-23
+// in all; a product below the smallest normal number lets the weight pass).
+struct Best {
+  uint64_t key = 0;
+  float least = 0.f;
+  __device__ __forceinline__ bool may(float weight, float noise) const {
+    return weight > 0.f && !(weight < least * noise - 2e-38f);
+  }
+  // eight columns from v: weights a - b, or a without column `taken`
+  template <bool DIFF>
+  __device__ __forceinline__ void vector(float (&a)[8], const float (&b)[8], const float (&n)[8], int64_t v, int64_t taken) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (DIFF) a[i] = __fsub_rn(a[i], b[i]);
+      else if (v + i == taken) a[i] = 0.f;
+      any |= may(a[i], n[i]);
+    }
+    if (any) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (may(a[i], n[i])) take(a[i], n[i], v + i);
+    }
+  }
+  __device__ __forceinline__ void take(float weight, float noise, int64_t v) {
+    const uint64_t k = key_of(weight, noise, v);
+    if (k > key) {
+      key = k;
+      least = __uint_as_float((uint32_t)(k >> 32)) * (1.f - 0x1p-20f);
+      if (!(least < 3e38f)) least = 3e38f;  // an infinite score: its product with a noise of zero stays a number
+    }
+  }
+};
+
 // The best key of columns [lo, hi): weights p, or max(p - q, 0), or p without
 // column `taken`.
-template <typename T, bool VEC>
+template <typename T, bool VEC, bool DIFF>
 __device__ __forceinline__ uint64_t scan(const T* __restrict__ p, const T* __restrict__ q, int64_t taken,
                                          const float* __restrict__ e, int64_t lo, int64_t hi) {
-  uint64_t best = 0;
+  Best best;
   if (VEC) {  // lo, hi multiples of 8, rows at 16-byte boundaries
-#pragma unroll 2
-    for (int64_t v = lo + threadIdx.x * 8; v < hi; v += kVerifyThreads * 8) {
+    constexpr int U = 2;  // vectors of eight in flight
+    const int64_t STEP = blockDim.x * 8;
+    int64_t v = lo + threadIdx.x * 8;
+    for (; v + (U - 1) * STEP < hi; v += U * STEP) {
+      float a[U][8], b[U][8], n[U][8];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        load8(p + v + u * STEP, a[u]);
+        load8(e + v + u * STEP, n[u]);
+        if (DIFF) load8(q + v + u * STEP, b[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) best.vector<DIFF>(a[u], b[u], n[u], v + u * STEP, taken);
+    }
+    for (; v < hi; v += STEP) {
       float a[8], b[8], n[8];
       load8(p + v, a);
       load8(e + v, n);
-      if (q) load8(q + v, b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = q ? __fsub_rn(a[i], b[i]) : (v + i == taken ? 0.f : a[i]);
-        best = best_of(best, key_of(w, n[i], v + i));
-      }
+      if (DIFF) load8(q + v, b);
+      best.vector<DIFF>(a, b, n, v, taken);
     }
   } else {
 #pragma unroll 4
-    for (int64_t v = lo + threadIdx.x; v < hi; v += kVerifyThreads) {
-      const float a = to_f32<T>(p[v]);
-      const float w = q ? __fsub_rn(a, to_f32<T>(q[v])) : (v == taken ? 0.f : a);
-      best = best_of(best, key_of(w, e[v], v));
+    for (int64_t v = lo + threadIdx.x; v < hi; v += blockDim.x) {
+      float w = to_f32<T>(p[v]);
+      if (DIFF) w = __fsub_rn(w, to_f32<T>(q[v]));
+      else if (v == taken) w = 0.f;
+      const float n = e[v];
+      if (best.may(w, n)) best.take(w, n, v);
     }
   }
-  return best;
+  return best.key;
 }
 
 // grid (cluster, seqs)
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs a) {
-  __shared__ uint64_t warp_best[kVerifyThreads / 32];
+__global__ void __launch_bounds__(kVerifyMostThreads, 2) verify_kernel(const VerifyArgs a) {
+  __shared__ uint64_t warp_best[kVerifyMostThreads / 32];
   __shared__ uint64_t cta_best[2][kVerifyMostCluster];  // written by the cluster's CTAs
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x, size = gridDim.x;
@@ -117,16 +164,16 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   const float* e = a.noise + b * a.noise_stride;
   uint64_t best = 0;
   for (int pass = accepted == count ? 1 : 0; pass < 2; ++pass) {
-    if (pass == 0)
-      best = scan<T, VEC>(p, a.draft ? draft + accepted * a.draft_row : nullptr, a.draft ? -1 : tokens[accepted], e, lo, hi);
+    if (pass == 0 && a.draft)
+      best = scan<T, VEC, true>(p, draft + accepted * a.draft_row, -1, e, lo, hi);
     else
-      best = scan<T, VEC>(p, nullptr, -1, e, lo, hi);
+      best = scan<T, VEC, false>(p, nullptr, pass == 0 ? tokens[accepted] : -1, e, lo, hi);
 #pragma unroll
     for (int o = 16; o; o >>= 1) best = best_of(best, __shfl_xor_sync(FULL, best, o));
     if (lane == 0) warp_best[warp] = best;
     __syncthreads();
     if (warp == 0) {
-      best = lane < kVerifyThreads / 32 ? warp_best[lane] : 0;
+      best = lane < blockDim.x / 32 ? warp_best[lane] : 0;
 #pragma unroll
       for (int o = 8; o; o >>= 1) best = best_of(best, __shfl_xor_sync(FULL, best, o));
       if (lane < size) {  // to slot `rank` of the lane-th CTA
@@ -143,23 +190,37 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const VerifyArgs
   }
   if (rank != 0) return;
   const int32_t next = best ? (int32_t)~(uint32_t)best : 0;
-  for (int i = tid; i <= a.drafts; i += kVerifyThreads)
+  for (int i = tid; i <= a.drafts; i += blockDim.x)
     a.out[b * (a.drafts + 1) + i] = i < accepted ? tokens[i] : (i == accepted ? next : -1);
   if (tid == 0) a.accepted[b] = accepted;
 }
 
 template <typename T, bool VEC>
 int launch_verify(const VerifyArgs& a, int64_t seqs, cudaStream_t stream) {
-  constexpr int CLUSTER = 8;
+  // eight CTAs of 256 threads a sequence; sixteen of 512 while that leaves SMs
+  // without one
+  const bool few = seqs * 8 <= sm_count();
+  const int cluster = few ? 16 : 8;
+  static bool allowed[kMaxDevices] = {};
+  const int dev = device_index();
+  if (!allowed[dev]) {  // clusters of more than eight are opted into, once for each device
+    const cudaError_t e = cudaFuncSetAttribute(verify_kernel<T, VEC>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      set_last_cuda_error(e);
+      return TQ_E_CUDA;
+    }
+    allowed[dev] = true;
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(CLUSTER, (unsigned)seqs);
-  cfg.blockDim = dim3(kVerifyThreads);
+  cfg.gridDim = dim3(cluster, (unsigned)seqs);
+  cfg.blockDim = dim3(few ? 512 : 256);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = CLUSTER;
+  attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;

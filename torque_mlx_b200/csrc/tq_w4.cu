@@ -26,16 +26,16 @@ namespace tq {
 constexpr int kW4Threads = 512;
 constexpr int kW4Warps = kW4Threads / 32;
 constexpr int kW4MaxTokens = TQ_W4_MAX_TOKENS;
-constexpr int kW4Block = 64;  // columns of a fragment block
+constexpr int kW4Block = 128;  // columns of a fragment block
 constexpr int kW4Smem = 227 * 1024 - 4096;  // dynamic; the static arrays take the rest
 
-constexpr int kW4Stages = 8;  // fragments of a warp's ring
+constexpr int kW4Stages = 5;  // fragments of a warp's ring
 
 enum W4Input { kW4Plain = 0, kW4F32 = 1, kW4Rms = 2, kW4Silu = 3 };
 
 struct W4Args {
-  const uint4* codes;     // [tiles][blocks][32]: word j of lane's four = step j of 16 columns
-  const uint8_t* scales;  // [tiles][scale blocks][8][sg][2] bf16: rows g and g + 8
+  const uint4* codes;     // [tiles][blocks][2][32]: word j of half i = columns 64 i + 16 j of the block
+  const uint8_t* scales;  // [tiles][blocks][8][groups of a block][2] bf16: rows g and g + 8
   const void* x;
   const void* norm_w;
   const void* residual;
@@ -54,17 +54,12 @@ struct W4Args {
 inline bool valid_group(int g) { return g == 32 || g == 64 || g == 128; }
 inline int64_t w4_tiles(int64_t n) { return (n + 15) / 16; }
 inline int64_t w4_blocks(int64_t k) { return (k + kW4Block - 1) / kW4Block; }
-// scale entries along the columns: one for each block, or for each two blocks (group 128)
-inline int64_t w4_scale_blocks(int64_t k, int group) { return group == 128 ? (w4_blocks(k) + 1) / 2 : w4_blocks(k); }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp8(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+template <int BYTES> __device__ __forceinline__ void cp_scales(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void w4_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void w4_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -149,11 +144,11 @@ __device__ __forceinline__ void w4_input(const W4Args& a, int64_t m, int64_t k0,
   }
 }
 
-// NT tiles of eight tokens, SG groups of a block (2 for groups of 32).
+// NT tiles of eight tokens, SG groups of a block.
 template <int NT, int SG, typename T>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   using Math = W4Math<T>;
-  constexpr int UNIT = 512 + 32 * SG, STAGES = kW4Stages;
+  constexpr int UNIT = 1024 + 32 * SG, STAGES = kW4Stages;
   extern __shared__ __align__(128) uint8_t w4_smem[];
   __shared__ float red[kW4Warps][kW4MaxTokens];
   __shared__ float inv_rms[kW4MaxTokens];
@@ -161,7 +156,7 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c = lane & 3;
   uint8_t* ring = w4_smem + warp * STAGES * UNIT;
   float4* pieces = reinterpret_cast<float4*>(w4_smem + kW4Warps * STAGES * UNIT);  // [warps][NT][32]
-  uint8_t* xs = reinterpret_cast<uint8_t*>(pieces + kW4Warps * NT * 32);           // [block][half][token][4] x 16 bytes
+  uint8_t* xs = reinterpret_cast<uint8_t*>(pieces + kW4Warps * NT * 32);           // [block][4][token][4] x 16 bytes
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
   const int M = a.tokens;
   const int b_lo = blockIdx.y * a.slab, b_hi = min(a.blocks, b_lo + a.slab), nb = b_hi - b_lo;
@@ -175,25 +170,23 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
   grid_wait();
   // ---- the ring's first fragments ----
   int left = steps, in_block = first_block;
-  const uint8_t* src = reinterpret_cast<const uint8_t*>(a.codes) +
-                       (((int64_t)first_tile * a.blocks + b_lo + first_block) * 32 + lane) * 16;
-  const int scale_blocks = a.group == 128 ? (a.blocks + 1) / 2 : a.blocks;
-  const uint8_t* ssrc = a.scales + (int64_t)first_tile * scale_blocks * (32 * SG) + g * (4 * SG);
+  const int64_t first_unit = (int64_t)first_tile * a.blocks + b_lo + first_block;
+  const uint8_t* src = reinterpret_cast<const uint8_t*>(a.codes) + first_unit * 1024 + lane * 16;
+  const uint8_t* ssrc = a.scales + first_unit * (32 * SG) + g * (4 * SG);
+  const int64_t skip = a.blocks - nb;  // blocks of other slabs between two tiles
   auto issue = [&](int st) {
     if (left > 0) {
       const uint32_t dst = ring_at + st * UNIT;
       cp16(dst + lane * 16, src);
-      if (c == 0) {
-        const uint8_t* s = ssrc + (int64_t)(a.group == 128 ? (b_lo + in_block) >> 1 : b_lo + in_block) * (32 * SG);
-        if (SG == 2) cp8(dst + 512 + g * 8, s);
-        else cp4(dst + 512 + g * 4, s);
-      }
+      cp16(dst + 512 + lane * 16, src + 512);
+      if (c == 0) cp_scales<4 * SG>(dst + 1024 + g * (4 * SG), ssrc);
       --left;
-      src += 512;
-      if (++in_block == nb) {
+      src += 1024;
+      ssrc += 32 * SG;
+      if (skip && ++in_block == nb) {
         in_block = 0;
-        src += (int64_t)(a.blocks - nb) * 512;
-        ssrc += (int64_t)scale_blocks * (32 * SG);
+        src += skip * 1024;
+        ssrc += skip * (32 * SG);
       }
     }
     w4_commit();
@@ -230,8 +223,8 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     const int m = i / pieces8, at = i - m * pieces8;
     float f[8];
     w4_input<T>(a, m, k_lo + at * 8, a.mode == kW4Rms ? inv_rms[m] : 0.f, vec, f);
-    const int b = at / 8, j = at % 8 / 2, half = at & 1;
-    uint8_t* dst = xs + ((b * 2 + (j >> 1)) * M + m) * 64 + ((j & 1) * 4 + half * 2) * 2;
+    const int b = at / 16, j = at % 16 / 2, half = at & 1;
+    uint8_t* dst = xs + ((b * 4 + (j >> 1)) * M + m) * 64 + ((j & 1) * 4 + half * 2) * 2;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const T lo = from_f32<T>(f[2 * q]), hi = from_f32<T>(f[2 * q + 1]);
@@ -270,64 +263,77 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
       }
   };
   clear();
-  int tile = first_tile, b = first_block, st = 0;
+  int tile = first_tile, b = first_block;
   bool begun = first_block == 0;  // the tile's first block was this warp's
-  const uint4* xp = reinterpret_cast<const uint4*>(xs) + g * 4 + c;
-  for (int it = 0; it < steps; ++it) {
-    w4_wait<STAGES - 2>();
-    __syncwarp();
-    issue(st == 0 ? STAGES - 1 : st - 1);
-    const uint8_t* unit = ring + st * UNIT;
-    const uint4 w4 = *reinterpret_cast<const uint4*>(unit + lane * 16);
-    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-    uint32_t xb[NT][8];
+  // a lane past the last token reads that one again: its sums are not used
+  const uint4 *x0[NT], *xp[NT];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-      if (nt * 8 + g < M) {
-        const uint4* p = xp + b * (M * 8) + nt * 32;
-        lo = p[0];
-        hi = p[M * 4];
-      }
-      xb[nt][0] = lo.x, xb[nt][1] = lo.y, xb[nt][2] = lo.z, xb[nt][3] = lo.w;
-      xb[nt][4] = hi.x, xb[nt][5] = hi.y, xb[nt][6] = hi.z, xb[nt][7] = hi.w;
-    }
-    const uint32_t* sp = reinterpret_cast<const uint32_t*>(unit + 512) + g * SG;
+  for (int nt = 0; nt < NT; ++nt) {
+    x0[nt] = reinterpret_cast<const uint4*>(xs) + min(nt * 8 + g, M - 1) * 4 + c;
+    xp[nt] = x0[nt] + (int64_t)first_block * M * 16;
+  }
+  for (int it = 0; it < steps; it += STAGES) {
 #pragma unroll
-    for (int s = 0; s < SG; ++s) {
+    for (int st = 0; st < STAGES; ++st) {
+      if (it + st >= steps) break;
+      w4_wait<STAGES - 2>();
+      __syncwarp();
+      issue(st == 0 ? STAGES - 1 : st - 1);
+      const uint8_t* unit = ring + st * UNIT;
+      const uint4 wl = *reinterpret_cast<const uint4*>(unit + lane * 16);
+      const uint4 wh = *reinterpret_cast<const uint4*>(unit + 512 + lane * 16);
+      const uint32_t w[8] = {wl.x, wl.y, wl.z, wl.w, wh.x, wh.y, wh.z, wh.w};
+      uint32_t two[SG];  // scales of rows g and g + 8
+#pragma unroll
+      for (int s = 0; s < SG; ++s) two[s] = reinterpret_cast<const uint32_t*>(unit + 1024)[g * SG + s];
       float sum[NT][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int i = 0; i < 4; ++i) {  // 32 columns
+        uint4 x[NT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[nt][i] = 0.f;
+        for (int nt = 0; nt < NT; ++nt) {
+          x[nt] = xp[nt][i * (M * 4)];
+        }
+        if (i % (4 / SG) == 0) {
 #pragma unroll
-      for (int j = s * 4 / SG; j < (s + 1) * 4 / SG; ++j) {
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[nt][k] = 0.f;
+        }
         uint32_t f[4];
-        Math::expand(w[j], f);
+        Math::expand(w[2 * i], f);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) Math::mma(sum[nt], f, xb[nt][2 * j], xb[nt][2 * j + 1]);
+        for (int nt = 0; nt < NT; ++nt) Math::mma(sum[nt], f, x[nt].x, x[nt].y);
+        Math::expand(w[2 * i + 1], f);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) Math::mma(sum[nt], f, x[nt].z, x[nt].w);
+        if ((i + 1) % (4 / SG) == 0) {
+          const uint32_t s2 = two[i / (4 / SG)];
+          const float s0 = __uint_as_float(s2 << 16), s1 = __uint_as_float(s2 & 0xffff0000u);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[nt][k] = fmaf(k < 2 ? s0 : s1, sum[nt][k], acc[nt][k]);
+        }
       }
-      const uint32_t two = sp[s];
-      const float s0 = __uint_as_float(two << 16), s1 = __uint_as_float(two & 0xffff0000u);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) xp[nt] += M * 16;
+      if (++b == nb) {  // the tile ends here
+        if (begun) {
+          output(tile);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[nt][i] = fmaf(i < 2 ? s0 : s1, sum[nt][i], acc[nt][i]);
-    }
-    st = st + 1 == STAGES ? 0 : st + 1;
-    if (++b == nb) {  // the tile ends here
-      if (begun) {
-        output(tile);
-      } else {
+          for (int nt = 0; nt < NT; ++nt)
+            pieces[(warp * NT + nt) * 32 + lane] = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
+          if (lane == 0) piece_tile[warp] = tile;
+        }
+        clear();
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          pieces[(warp * NT + nt) * 32 + lane] = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-        if (lane == 0) piece_tile[warp] = tile;
+        for (int nt = 0; nt < NT; ++nt) xp[nt] = x0[nt];
+        b = 0;
+        ++tile;
+        begun = true;
       }
-      clear();
-      b = 0;
-      ++tile;
-      begun = true;
     }
   }
   if (b != 0 && !begun) {  // the run lies within one tile
@@ -382,9 +388,9 @@ __global__ void __launch_bounds__(256) w4_layout_kernel(const uint8_t* __restric
                                                         uint32_t* __restrict__ out, uint16_t* __restrict__ sout) {
   grid_wait();
   const int64_t stride = (int64_t)gridDim.x * 256, row_bytes = (k + 1) / 2;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tiles * blocks * 128; i += stride) {
-    const int j = (int)(i & 3), lane = (int)(i >> 2) & 31, g = lane >> 2, c = lane & 3;
-    const int64_t unit = i >> 7, tile = unit / blocks, b = unit - tile * blocks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tiles * blocks * 256; i += stride) {
+    const int j = (int)(i & 3) + ((int)(i >> 7) & 1) * 4, lane = (int)(i >> 2) & 31, g = lane >> 2, c = lane & 3;
+    const int64_t unit = i >> 8, tile = unit / blocks, b = unit - tile * blocks;
     uint32_t w = 0;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
@@ -401,13 +407,13 @@ __global__ void __launch_bounds__(256) w4_layout_kernel(const uint8_t* __restric
     }
     out[i] = w;
   }
-  const int sg = group == 32 ? 2 : 1;
-  const int64_t sblocks = group == 128 ? (blocks + 1) / 2 : blocks, groups = (k + group - 1) / group;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tiles * sblocks * 16 * sg; i += stride) {
+  const int sg = kW4Block / group;
+  const int64_t groups = (k + group - 1) / group;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tiles * blocks * 16 * sg; i += stride) {
     const int which = (int)(i & 1);
     const int64_t v = i >> 1;
     const int s = (int)(v % sg), g = (int)(v / sg) & 7;
-    const int64_t at = v / sg / 8, tile = at / sblocks, b = at - tile * sblocks;
+    const int64_t at = v / sg / 8, tile = at / blocks, b = at - tile * blocks;
     const int64_t row = tile * 16 + g + 8 * which, grp = b * sg + s;
     sout[i] = row < n && grp < groups ? scales[row * groups + grp] : 0;
   }
@@ -450,14 +456,13 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint32_t* __re
                                                             int group, int64_t tiles, int64_t blocks,
                                                             T* __restrict__ out) {
   grid_wait();
-  const int sg = group == 32 ? 2 : 1;
-  const int64_t sblocks = group == 128 ? (blocks + 1) / 2 : blocks;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tiles * blocks * 128; i += (int64_t)gridDim.x * 256) {
-    const int j = (int)(i & 3), lane = (int)(i >> 2) & 31, g = lane >> 2, c = lane & 3;
-    const int64_t unit = i >> 7, tile = unit / blocks, b = unit - tile * blocks;
+  const int sg = kW4Block / group;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tiles * blocks * 256; i += (int64_t)gridDim.x * 256) {
+    const int j = (int)(i & 3) + ((int)(i >> 7) & 1) * 4, lane = (int)(i >> 2) & 31, g = lane >> 2, c = lane & 3;
+    const int64_t unit = i >> 8, tile = unit / blocks, b = unit - tile * blocks;
     const uint32_t w = codes[i];
-    const int s = sg == 2 ? j >> 1 : 0;
-    const int64_t sb = (tile * sblocks + (group == 128 ? b >> 1 : b)) * 8 + g;
+    const int s = j * 16 / group;
+    const int64_t sb = unit * 8 + g;
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       int r, q;
@@ -476,15 +481,15 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(const uint32_t* __re
 // ---------------------------------------------------------------------------
 inline int w4_nt(int tokens) { return tokens <= 8 ? 1 : tokens <= 16 ? 2 : 4; }
 inline size_t w4_fixed_smem(int nt, int sg) {
-  return (size_t)kW4Warps * (kW4Stages * (512 + 32 * sg) + nt * 32 * sizeof(float4));
+  return (size_t)kW4Warps * (kW4Stages * (1024 + 32 * sg) + nt * 32 * sizeof(float4));
 }
 // Column blocks of a slab: all of them where x' fits beside the ring, else
-// equal shares (an even number, so that groups of 128 stay whole).
+// equal shares.
 inline int64_t w4_slab(int64_t blocks, int tokens) {
-  const int64_t room = (int64_t)(kW4Smem - w4_fixed_smem(w4_nt(tokens), 2)) / (2 * kW4Block * tokens);
+  const int64_t room = (int64_t)(kW4Smem - w4_fixed_smem(w4_nt(tokens), 4)) / (2 * kW4Block * tokens);
   if (blocks <= room) return blocks;
-  const int64_t slabs = (blocks + room / 2 * 2 - 1) / (room / 2 * 2), even = (blocks + slabs - 1) / slabs;
-  return (even + 1) / 2 * 2;
+  const int64_t slabs = (blocks + room - 1) / room;
+  return (blocks + slabs - 1) / slabs;
 }
 
 template <int NT, int SG, typename T>
@@ -509,12 +514,16 @@ int launch_w4(const W4Args& a, cudaStream_t stream) {
   return launch_dependent(kernel, dim3(x, slabs), dim3(kW4Threads), smem, stream, a);
 }
 
+template <int NT, typename T>
+int launch_w4_group(const W4Args& a, cudaStream_t stream) {
+  if (a.group == 128) return launch_w4<NT, 1, T>(a, stream);
+  return a.group == 64 ? launch_w4<NT, 2, T>(a, stream) : launch_w4<NT, 4, T>(a, stream);
+}
+
 template <typename T>
 int launch_w4_all(const W4Args& a, int nt, cudaStream_t stream) {
-  const bool two = a.group == 32;
-  if (nt == 1) return two ? launch_w4<1, 2, T>(a, stream) : launch_w4<1, 1, T>(a, stream);
-  if (nt == 2) return two ? launch_w4<2, 2, T>(a, stream) : launch_w4<2, 1, T>(a, stream);
-  return two ? launch_w4<4, 2, T>(a, stream) : launch_w4<4, 1, T>(a, stream);
+  if (nt == 1) return launch_w4_group<1, T>(a, stream);
+  return nt == 2 ? launch_w4_group<2, T>(a, stream) : launch_w4_group<4, T>(a, stream);
 }
 
 template <typename T>
@@ -541,7 +550,7 @@ int gemv_w4(W4Args a, int64_t tokens, void* workspace, cudaStream_t stream) {
 
 inline int check_w4(int64_t n, int64_t k, int group) {
   if (!valid_group(group) || n <= 0 || k <= 0) return TQ_E_SHAPE;
-  if (w4_tiles(n) > INT32_MAX / 2 || w4_blocks(k) > INT32_MAX / 64) return TQ_E_SHAPE;
+  if (w4_tiles(n) > INT32_MAX / 2 || w4_blocks(k) > INT32_MAX / 256) return TQ_E_SHAPE;
   return TQ_OK;
 }
 
@@ -555,8 +564,8 @@ int tq_w4_sizes(int64_t n, int64_t k, int group_size, size_t* code_bytes, size_t
   const int st = check_w4(n, k, group_size);
   if (st != TQ_OK) return st;
   if (!code_bytes || !scale_bytes) return TQ_E_ARG;
-  *code_bytes = (size_t)w4_tiles(n) * w4_blocks(k) * 512;
-  *scale_bytes = (size_t)w4_tiles(n) * w4_scale_blocks(k, group_size) * 32 * (group_size == 32 ? 2 : 1);
+  *code_bytes = (size_t)w4_tiles(n) * w4_blocks(k) * 1024;
+  *scale_bytes = (size_t)w4_tiles(n) * w4_blocks(k) * 32 * (kW4Block / group_size);
   return TQ_OK;
 }
 

@@ -47,13 +47,13 @@ class _Batch(Structure):
 _scratch: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def scratch(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
-    """Workspace of one stream, grown as needed: calls on a stream are ordered
-    and share it, calls on different streams do not meet.  A captured call
-    takes memory of its graph's pool instead."""
+def scratch(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Workspace of ``device``'s current stream, grown as needed: calls on a
+    stream are ordered and share it, calls on different streams do not meet.  A
+    captured call takes memory of its graph's pool instead."""
     if torch.cuda.is_current_stream_capturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, stream)
+    key = (device.index, _lib.stream_of(device.index))
     buf = _scratch.get(key)
     if buf is None or buf.numel() < nbytes:
         buf = _scratch[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
@@ -62,13 +62,13 @@ def scratch(nbytes: int, device: torch.device, stream: int) -> torch.Tensor:
 
 def rows_of(x: torch.Tensor) -> torch.Tensor:
     """``x`` with contiguous rows at 16-byte boundaries, copied only where it has none."""
-    item = x.element_size()
-    inner = 1
-    for n, st in zip(reversed(x.shape[1:]), reversed(x.stride()[1:])):
-        if n != 1 and st != inner:
-            return x.contiguous()
-        inner *= n
-    if x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) * item % 16):
+    if not x.is_contiguous():
+        inner = 1
+        for n, st in zip(reversed(x.shape[1:]), reversed(x.stride()[1:])):
+            if n != 1 and st != inner:
+                return x.contiguous()
+            inner *= n
+    if x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) * x.element_size() % 16):
         return x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -122,7 +122,7 @@ class PagedKV8Cache:
     def _bind(self, kp: torch.Tensor, vp: torch.Tensor, ks: torch.Tensor, vs: torch.Tensor) -> None:
         self.key_pages, self.value_pages, self.key_scales, self.value_scales = kp, vp, ks, vs
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = (int(n) for n in kp.shape)
-        self.device = kp.device
+        self.device, self._index = kp.device, kp.get_device()
         self._kv = _KV(kp.data_ptr(), vp.data_ptr(), ks.data_ptr(), vs.data_ptr(), self.num_pages, self.kv_heads,
                        self.page_size, self.head_dim)
         self._kv_ref = byref(self._kv)
@@ -131,14 +131,16 @@ class PagedKV8Cache:
     # ----------------------------------------------------------------- batch
     def _batch(self, rows: int, lengths: torch.Tensor, block_table: torch.Tensor, token_starts: torch.Tensor | None,
                max_new_tokens: int | None) -> _Batch:
-        dev = self.device
-        if lengths.dtype != torch.int32 or lengths.dim() != 1 or lengths.device != dev or not lengths.is_contiguous():
+        dev, index = self.device, self._index
+        if (lengths.dtype is not torch.int32 or lengths.dim() != 1 or lengths.get_device() != index
+                or not lengths.is_contiguous()):
             raise ValueError(f"lengths must be contiguous int32 [seqs] on {dev}")
-        seqs = lengths.shape[0]
+        seqs = lengths.numel()
         if seqs > MAX_SEQS:
             raise ValueError(f"at most {MAX_SEQS} sequences in a batch, got {seqs}")
-        if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.device != dev
-                or block_table.shape[0] != seqs or (block_table.shape[1] > 1 and block_table.stride(1) != 1)):
+        table_seqs, width = block_table.shape if block_table.dim() == 2 else (-1, 0)
+        if (block_table.dtype is not torch.int32 or table_seqs != seqs or block_table.get_device() != index
+                or (width > 1 and block_table.stride(1) != 1)):
             raise ValueError(f"block_table must be int32 [{seqs}, pages] on {dev} with contiguous rows")
         starts = None
         if token_starts is None:
@@ -146,14 +148,14 @@ class PagedKV8Cache:
                 raise ValueError(f"without token_starts every sequence brings one row: {seqs} sequences, {rows} rows")
             most = 1
         else:
-            if (token_starts.dtype != torch.int32 or token_starts.dim() != 1 or token_starts.device != dev
-                    or token_starts.shape[0] != seqs + 1 or not token_starts.is_contiguous()):
+            if (token_starts.dtype is not torch.int32 or token_starts.dim() != 1
+                    or token_starts.get_device() != index or token_starts.numel() != seqs + 1
+                    or not token_starts.is_contiguous()):
                 raise ValueError(f"token_starts must be contiguous int32 [{seqs + 1}] on {dev}")
             starts = token_starts.data_ptr()
             most = rows if max_new_tokens is None else max_new_tokens
             if most < 0:
                 raise ValueError("max_new_tokens must not be negative")
-        width = block_table.shape[1]
         return _Batch(block_table.data_ptr(), lengths.data_ptr(), starts,
                       block_table.stride(0) if seqs > 1 else width, rows, width, seqs, min(most, rows))
 
@@ -176,8 +178,12 @@ class PagedKV8Cache:
         position has no table row is not written and its query is NaN; a row
         whose page is missing is not written."""
         lib = _lib.load()
+        if _lib.current_device() != self._index:
+            with torch.cuda.device(self.device):
+                return self.append(qkv, cos, sin, lengths=lengths, block_table=block_table, token_starts=token_starts,
+                                   max_new_tokens=max_new_tokens, interleaved=interleaved, out=out)
         d, Hkv = self.head_dim, self.kv_heads
-        if qkv.dim() != 2 or qkv.device != self.device:
+        if qkv.dim() != 2 or qkv.get_device() != self._index:
             raise ValueError(f"qkv must be [rows, (q_heads + {2 * Hkv}) * {d}] on {self.device}")
         rows, width = qkv.shape
         q_heads = width // d - 2 * Hkv
@@ -187,24 +193,26 @@ class PagedKV8Cache:
         batch = self._batch(rows, lengths, block_table, token_starts, max_new_tokens)
         rotary, positions, cp, sp = 0, 0, None, None
         if cos is not None or sin is not None:
-            if (cos is None or sin is None or cos.shape != sin.shape or cos.dim() != 2
-                    or cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.device != self.device
-                    or sin.device != self.device or not cos.is_contiguous() or not sin.is_contiguous()):
+            if (cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape
+                    or cos.dtype is not torch.float32 or sin.dtype is not torch.float32
+                    or cos.get_device() != self._index or sin.get_device() != self._index
+                    or not cos.is_contiguous() or not sin.is_contiguous()):
                 raise ValueError(f"cos and sin must be contiguous fp32 tables [positions, rotary_dim / 2] on {self.device}")
-            positions, rotary = cos.shape[0], 2 * cos.shape[1]
+            positions, rotary = cos.shape
+            rotary *= 2
             if rotary % 16 or rotary > d:
                 raise ValueError(f"rotary_dim must be a multiple of 16 up to {d}, got {rotary}")
             cp, sp = cos.data_ptr(), sin.data_ptr()
         qkv = rows_of(qkv)
         if out is None:
-            out = torch.empty((rows, q_heads, d), dtype=qkv.dtype, device=self.device)
-        elif (out.shape != (rows, q_heads, d) or out.dtype != qkv.dtype or out.device != self.device
+            out = qkv.new_empty((rows, q_heads, d))
+        elif (out.shape != (rows, q_heads, d) or out.dtype is not qkv.dtype or out.get_device() != self._index
               or not out.is_contiguous()):
             raise ValueError(f"out must be contiguous {qkv.dtype} [{rows}, {q_heads}, {d}]")
-        with torch.cuda.device(self.device):
-            _lib.check(lib.tq_paged_append(self._kv_ref, byref(batch), qkv.data_ptr(), code, qkv.stride(0), q_heads,
-                                           cp, sp, positions, rotary, int(interleaved), out.data_ptr(),
-                                           _lib.stream_ptr()), "paged append")
+        status = lib.tq_paged_append(self._kv_ref, byref(batch), qkv.data_ptr(), code, qkv.stride(0), q_heads, cp, sp,
+                                     positions, rotary, interleaved, out.data_ptr(), _lib.stream_of(self._index))
+        if status:
+            _lib.check(status, "paged append")
         return out
 
     # ---------------------------------------------------------------- attend
@@ -221,14 +229,20 @@ class PagedKV8Cache:
         ``max_context`` (a bound of any sequence's tokens, new ones included)
         sizes the launch; the result does not depend on it."""
         lib = _lib.load()
+        if _lib.current_device() != self._index:
+            with torch.cuda.device(self.device):
+                return self.attend(q, lengths=lengths, block_table=block_table, token_starts=token_starts,
+                                   max_new_tokens=max_new_tokens, max_context=max_context,
+                                   lengths_counted=lengths_counted, scale=scale, return_lse=return_lse, out=out)
         d = self.head_dim
-        if q.dim() != 3 or q.shape[2] != d or q.device != self.device:
+        rows, q_heads, width = q.shape if q.dim() == 3 else (0, 0, 0)
+        if width != d or q.get_device() != self._index:
             raise ValueError(f"q must be [rows, q_heads, {d}] on {self.device}")
-        rows, q_heads, _ = q.shape
         if q_heads == 0 or q_heads % self.kv_heads:
             raise ValueError(f"q_heads {q_heads} must be a positive multiple of kv_heads {self.kv_heads}")
-        if q.dtype != torch.bfloat16 and q.dtype != torch.float16:
-            raise ValueError(f"q must be float16 or bfloat16, got {q.dtype}")
+        dtype = q.dtype
+        if dtype is not torch.bfloat16 and dtype is not torch.float16:
+            raise ValueError(f"q must be float16 or bfloat16, got {dtype}")
         batch = self._batch(rows, lengths, block_table, token_starts, max_new_tokens)
         if max_context is None:
             max_context = batch.table_width * self.page_size
@@ -236,38 +250,50 @@ class PagedKV8Cache:
             raise ValueError("max_context must not be negative")
         q = rows_of(q)
         if out is None:
-            out = torch.empty((rows, q_heads, d), dtype=q.dtype, device=self.device)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != self.device or not out.is_contiguous():
-            raise ValueError(f"out must be contiguous {q.dtype} {tuple(q.shape)}")
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        elif (out.shape != (rows, q_heads, d) or out.dtype is not dtype or out.get_device() != self._index
+              or not out.is_contiguous()):
+            raise ValueError(f"out must be contiguous {dtype} {(rows, q_heads, d)}")
         lse = torch.empty((rows, q_heads), dtype=torch.float32, device=self.device) if return_lse else None
-        key = (q_heads, batch.max_new_tokens)
-        with torch.cuda.device(self.device):
-            need = self._need.get(key)
-            if need is None:
-                size = c_size_t()
-                _lib.check(lib.tq_paged_attend_workspace_size(self._kv_ref, *key, byref(size)), "paged attend")
-                need = self._need[key] = size.value
-            stream = _lib.stream_ptr()
-            ws = scratch(need, self.device, stream)
-            _lib.check(lib.tq_paged_attend(
-                self._kv_ref, byref(batch), q.data_ptr(), _lib.dtype_code(q.dtype), q.stride(0), q_heads,
-                int(lengths_counted), float(d ** -0.5 if scale is None else scale), max_context, out.data_ptr(),
-                _lib.ptr(lse), ws.data_ptr(), ws.numel(), stream), "paged attend")
+        need = self._workspace(q_heads, batch.max_new_tokens)
+        ws = scratch(need, self.device)
+        status = lib.tq_paged_attend(
+            self._kv_ref, byref(batch), q.data_ptr(), _lib.TQ_BF16 if dtype is torch.bfloat16 else _lib.TQ_F16,
+            q.stride(0), q_heads, lengths_counted, d ** -0.5 if scale is None else scale, max_context, out.data_ptr(),
+            None if lse is None else lse.data_ptr(), ws.data_ptr(), need, _lib.stream_of(self._index))
+        if status:
+            _lib.check(status, "paged attend")
         return (out, lse) if return_lse else out
+
+    def _workspace(self, q_heads: int, max_new_tokens: int) -> int:
+        """Bytes of an attention's workspace, asked once for each pair."""
+        key = (q_heads, max_new_tokens)
+        need = self._need.get(key)
+        if need is None:
+            size = c_size_t()
+            _lib.check(_lib.load().tq_paged_attend_workspace_size(self._kv_ref, q_heads, max_new_tokens, byref(size)),
+                       "paged attend")
+            need = self._need[key] = size.value
+        return need
 
     # ------------------------------------------------------------ dequantize
     def dequantize(self, page_ids: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16):
         """The values of pages: ``(keys, values)``, each ``[n, kv_heads,
         page_size, d]`` (tq_paged_dequantize); NaN for an id outside the pool."""
         lib = _lib.load()
-        if (page_ids.dtype != torch.int32 or page_ids.dim() != 1 or page_ids.device != self.device
+        if _lib.current_device() != self._index:
+            with torch.cuda.device(self.device):
+                return self.dequantize(page_ids, dtype=dtype)
+        if (page_ids.dtype is not torch.int32 or page_ids.dim() != 1 or page_ids.get_device() != self._index
                 or not page_ids.is_contiguous()):
             raise ValueError(f"page_ids must be contiguous int32 [n] on {self.device}")
         code = _lib.dtype_code(dtype)
-        both = torch.empty((2, page_ids.shape[0], self.kv_heads, self.page_size, self.head_dim), dtype=dtype,
-                           device=self.device)
-        k, v = both.unbind(0)
-        with torch.cuda.device(self.device):
-            _lib.check(lib.tq_paged_dequantize(self._kv_ref, page_ids.data_ptr(), page_ids.shape[0], k.data_ptr(),
-                                               v.data_ptr(), code, _lib.stream_ptr()), "paged dequantize")
+        n = page_ids.numel()
+        shape = (n, self.kv_heads, self.page_size, self.head_dim)
+        k = torch.empty(shape, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        status = lib.tq_paged_dequantize(self._kv_ref, page_ids.data_ptr(), n, k.data_ptr(), v.data_ptr(), code,
+                                         _lib.stream_of(self._index))
+        if status:
+            _lib.check(status, "paged dequantize")
         return k, v

@@ -26,8 +26,17 @@ class W4Weight:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, group_size: int):
         self.codes, self.scales = codes, scales
         self.n, self.k, self.group_size = n, k, group_size
-        self.device = codes.device
+        self.device, self._index = codes.device, codes.get_device()
         self._need: dict[int, int] = {}  # workspace by token count
+
+    def _workspace(self, tokens: int) -> int:
+        """Bytes of a product's workspace, asked once for each token count."""
+        need = self._need.get(tokens)
+        if need is None:
+            size = c_size_t()
+            _lib.check(_lib.load().tq_gemv_w4_workspace_size(self.n, self.k, tokens, byref(size)), "gemv_w4")
+            need = self._need[tokens] = size.value
+        return need
 
     @staticmethod
     def _check_sizes(n: int, k: int, group_size: int) -> tuple[int, int]:
@@ -102,20 +111,23 @@ def gemv_w4(weight: W4Weight, x: torch.Tensor, *, mode: str = "plain", norm_weig
     Returns ``[tokens, n]`` (or ``[n]``) in x's type (bf16 for "f32").  Made for
     few tokens: the weight is read once for each 32 of them."""
     lib = _lib.load()
+    if _lib.current_device() != weight._index:
+        with torch.cuda.device(weight.device):
+            return gemv_w4(weight, x, mode=mode, norm_weight=norm_weight, eps=eps, residual=residual, out=out)
     try:
         code = _MODES[mode]
     except KeyError as exc:
         raise ValueError(f"mode must be one of {sorted(_MODES)}") from exc
     k, n, dev = weight.k, weight.n, weight.device
     width = 2 * k if code == 3 else k
-    if x.dim() not in (1, 2) or x.shape[-1] != width or x.device != dev:
+    if x.dim() not in (1, 2) or x.shape[-1] != width or x.get_device() != weight._index:
         raise ValueError(f"gemv_w4: x must be [tokens, {width}] on {dev}, got {tuple(x.shape)}")
     dtype = x.dtype
     if code == 1:
-        if dtype != torch.float32:
+        if dtype is not torch.float32:
             raise ValueError(f"gemv_w4: x must be float32 in mode 'f32', got {dtype}")
         dtype = torch.bfloat16
-    elif dtype != torch.bfloat16 and not (code == 0 and dtype == torch.float16):
+    elif dtype is not torch.bfloat16 and not (code == 0 and dtype is torch.float16):
         raise ValueError(f"gemv_w4: x must be bfloat16{' or float16' if code == 0 else ''} in mode {mode!r}, got {dtype}")
     tokens = x.shape[0] if x.dim() == 2 else 1
     if width > 1 and x.stride(-1) != 1:
@@ -134,19 +146,15 @@ def gemv_w4(weight: W4Weight, x: torch.Tensor, *, mode: str = "plain", norm_weig
             raise ValueError(f"gemv_w4: residual must be contiguous {dtype} {shape} on {dev}")
         res = residual.data_ptr()
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
+        out = x.new_empty(shape) if dtype is x.dtype else torch.empty(shape, dtype=dtype, device=dev)
     elif out.dtype != dtype or out.numel() != tokens * n or out.device != dev or not out.is_contiguous():
         raise ValueError(f"gemv_w4: out must be contiguous {dtype} {shape} on {dev}")
-    need = weight._need.get(tokens)
-    if need is None:
-        size = c_size_t()
-        _lib.check(lib.tq_gemv_w4_workspace_size(n, k, tokens, byref(size)), "gemv_w4")
-        need = weight._need[tokens] = size.value
-    with torch.cuda.device(dev):
-        stream = _lib.stream_ptr()
-        ws = scratch(need, dev, stream) if need else None
-        _lib.check(lib.tq_gemv_w4(weight.codes.data_ptr(), weight.scales.data_ptr(), n, k, weight.group_size,
-                                  x.data_ptr(), _lib.TQ_F16 if dtype == torch.float16 else _lib.TQ_BF16,
-                                  x.stride(0) if x.dim() == 2 else width, code, norm, float(eps), res, out.data_ptr(),
-                                  tokens, _lib.ptr(ws), need, stream), "gemv_w4")
+    need = weight._workspace(tokens)
+    ws = scratch(need, dev).data_ptr() if need else None
+    status = lib.tq_gemv_w4(weight.codes.data_ptr(), weight.scales.data_ptr(), n, k, weight.group_size, x.data_ptr(),
+                            _lib.TQ_F16 if dtype is torch.float16 else _lib.TQ_BF16,
+                            x.stride(0) if x.dim() == 2 else width, code, norm, eps, res, out.data_ptr(), tokens, ws,
+                            need, _lib.stream_of(weight._index))
+    if status:
+        _lib.check(status, "gemv_w4")
     return out
