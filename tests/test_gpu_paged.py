@@ -515,3 +515,128 @@ def test_empty_calls():
     assert cache.attend(empty, lengths=lengths, block_table=table, token_starts=starts).shape == (0, 4, 64)
     assert cache.append(torch.empty(0, 8 * 64, device="cuda"), lengths=lengths, block_table=table,
                         token_starts=starts).shape == (0, 4, 64)
+
+
+# ---------------------------------------------------------------------------
+# many rows for each kv head: tiles of 128
+# ---------------------------------------------------------------------------
+MANY = [
+    # lens, new, page, q_heads, kv_heads, d
+    ([0], [129], 64, 2, 2, 128),
+    ([0, 5], [33, 1], 16, 1, 1, 64),
+    ([4000], [40], 128, 8, 2, 128),
+    ([777, 0, 130, 12], [0, 64, 1, 100], 32, 4, 1, 64),
+    ([250, 2000], [3, 90], 16, 16, 2, 256),
+    ([127, 128, 129], [128, 127, 129], 64, 2, 1, 128),
+    ([1], [300], 16, 12, 4, 64),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,new,page,hq,hkv,d", MANY)
+def test_many_rows_match_fp64(lens, new, page, hq, hkv, d, dtype):
+    cache, table = make_cache(31 + d, lens, new, page=page, kv_heads=hkv, d=d)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q = (2 * torch.randn(sum(new), hq, d, generator=g, device="cuda")).to(dtype)
+    for most in (None, max(a + b for a, b in zip(lens, new))):
+        out, lse = cache.attend(q, block_table=table, return_lse=True, max_context=most, **batch_args(lens, new))
+        check_attend(cache, table, q, lens, new, out, lse)
+
+
+def test_many_rows_counted_and_empty():
+    lens, new = [20, 0, 200], [50, 40, 60]
+    cache, table = make_cache(41, lens, new, page=16, kv_heads=2, d=64)
+    q = torch.randn(sum(new), 4, 64, device="cuda").to(torch.float16)
+    out, lse = cache.attend(q, block_table=table, lengths_counted=True, return_lse=True, **batch_args(lens, new))
+    check_attend(cache, table, q, lens, new, out, lse, counted=True)
+    assert float(out[:30].abs().max()) == 0 and bool((lse[:30] == -math.inf).all())
+    assert float(out[50:90].abs().max()) == 0 and bool((lse[50:90] == -math.inf).all())
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_many_rows_page_scales_far_apart(d):
+    lens, new = [200, 75], [60, 45]
+    cache, table = make_cache(42, lens, new, page=16, kv_heads=1, d=d, v_spread=2.0 ** 20)
+    cache.value_scales[table[0, 1].long()] = 0
+    cache.key_scales[table[0, 2].long()] = 0
+    cache.value_pages[table[0, 3].long()] = 128
+    cache.value_scales[table[0, 3].long()] = FLOOR
+    q = torch.randn(sum(new), 2, d, device="cuda").to(torch.bfloat16)
+    out, lse = cache.attend(q, block_table=table, return_lse=True, **batch_args(lens, new))
+    check_attend(cache, table, q, lens, new, out, lse)
+
+
+def test_many_rows_only_zero_values():
+    lens, new = [30], [40]
+    cache, table = make_cache(43, lens, new, page=16, kv_heads=1, d=64)
+    cache.value_pages.fill_(128)
+    cache.value_scales.fill_(FLOOR)
+    q = torch.randn(40, 2, 64, device="cuda").to(torch.bfloat16)
+    out, lse = cache.attend(q, block_table=table, return_lse=True, **batch_args(lens, new))
+    assert float(out.abs().max()) == 0
+    _, want, _ = attend64(cache, table, q, lens, new)
+    assert bool(((lse.double() - want).abs() <= 2e-5 * (1 + want.abs())).all())
+
+
+def test_many_rows_missing_pages_garbage_and_nonfinite_rows():
+    lens, new = [100, 40], [50, 70]
+    cache, table = make_cache(44, lens, new, page=16, kv_heads=2, d=64)
+    used = table[table >= 0].long()
+    other = torch.ones(cache.num_pages, dtype=torch.bool, device="cuda")
+    other[used] = False
+    cache.key_scales[other] = math.nan
+    cache.value_scales[other] = math.nan
+    cache.value_pages[table[0, 9].long(), :, 6:] = 255  # past the end
+    table[0, 1] = -1
+    table[1, 4] = cache.num_pages
+    ref = table.clone()
+    ref[1, 4] = -1
+    q = torch.randn(sum(new), 4, 64, device="cuda").to(torch.float16)
+    out, lse = cache.attend(q, block_table=table, return_lse=True, **batch_args(lens, new))
+    check_attend(cache, ref, q, lens, new, out, lse)
+    bad = q.clone()
+    bad[7, 1, 5] = math.nan
+    again = cache.attend(bad, block_table=table, **batch_args(lens, new))
+    assert bool(again[7, 1].isnan().all())
+    keep = torch.ones(out.shape[:2], dtype=torch.bool, device="cuda")
+    keep[7, 1] = False
+    assert torch.equal(again[keep], out[keep])
+
+
+def test_many_rows_scales_of_either_sign_stride_stream_graph_and_repeats():
+    lens, new = [300, 20], [61, 35]
+    cache, table = make_cache(45, lens, new, page=64, kv_heads=2, d=128)
+    wide = torch.randn(sum(new), 3, 8, 128, device="cuda").to(torch.bfloat16)
+    q = wide[:, 1]
+    args = batch_args(lens, new)
+    for scale in (0.05, -0.05, 0.0):
+        check_attend(cache, table, q, lens, new, cache.attend(q, block_table=table, scale=scale, **args), scale=scale)
+    want = cache.attend(q.contiguous(), block_table=table, **args)
+    assert torch.equal(cache.attend(q, block_table=table, **args), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            assert torch.equal(cache.attend(q, block_table=table, **args), want)
+    side.synchronize()
+    static = torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.attend(q, block_table=table, out=static, **args)
+    args["lengths"][0] = 299
+    graph.replay()
+    check_attend(cache, table, q, [299, 20], new, static)
+
+
+def test_many_rows_large_and_small_queries():
+    lens, new = [90], [40]
+    cache, table = make_cache(46, lens, new, page=32, kv_heads=1, d=128)
+    q = torch.randn(40, 2, 128, device="cuda")
+    q[:20] *= 2.0 ** 40
+    q[20:] *= 2.0 ** -40
+    q = q.to(torch.bfloat16)
+    for scale, rows in ((2.0 ** -43, slice(0, 20)), (2.0 ** 37, slice(20, 40))):
+        out = cache.attend(q, block_table=table, scale=scale, **batch_args(lens, new))
+        want, _, size = attend64(cache, table, q, lens, new, scale=scale)
+        tol = size[rows] + 2.0 ** -8 * want[rows].abs() + 1e-6
+        assert bool(((out[rows].double() - want[rows]).abs() <= tol).all())

@@ -18,7 +18,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libtorque_b200.so"
 SOURCES = ["tq_append.cu", "tq_decode.cu", "tq_decode_mma.cu", "tq_glue.cu", "tq_paged.cu",
-           "tq_paged_attend.cu", "tq_peer.cu", "tq_verify.cu", "tq_w4.cu"]
+           "tq_paged_attend.cu", "tq_paged_prefill.cu", "tq_peer.cu", "tq_verify.cu", "tq_w4.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -8,8 +8,9 @@
 // w_j = 2^(s_j + log2(scale_v) - m2), whose reference m2 is kept apart from
 // the softmax's own m, so that pages of very different scale neither overflow
 // nor vanish.  A bf16 query is multiplied by a power of two for each row that
-// takes its largest element to 2^13: fp16 then holds it exactly (elements
-// 2^-27 of the largest and below excepted).  Only the weights w are rounded,
+// takes its largest element to [2^12, 2^13): fp16 then holds it exactly
+// (elements under 2^-30 of the largest are off by 2^-38 of it, less than the
+// roundings of an fp32 product with it).  Only the weights w are rounded,
 // to fp16; scores, m, m2 and all sums stay in fp32.
 //
 // Bound: a decode step reads each code once.  At 148 SMs and the measured
@@ -23,7 +24,7 @@
 // CTAs, whatever the sequences' lengths (read on the device, so a captured
 // step follows them).  A unit that falls within one CTA is finished there; the
 // parts of a divided one meet in a second launch.
-#include "tq_paged.cuh"
+#include "tq_paged_attend.cuh"
 
 namespace tq {
 
@@ -32,96 +33,7 @@ constexpr int kAttendThreads = kAttendWarps * 32;
 constexpr int kChunk = 16;    // tokens of a ring stage
 constexpr int kMinChunks = 8; // smallest share of a CTA
 constexpr int kWholeChunks = 32;
-constexpr float kNoScore = -1e30f;  // finite, so that differences of two of them are not NaN
-constexpr float kLazy = 8.f;  // a score may pass its reference by 2^8 before the sums are rescaled
 
-struct AttendArgs {
-  tq_paged_kv kv;
-  tq_paged_batch bt;
-  const void* q;
-  void* out;
-  float* lse;
-  float* part_o;   // [ctas][2][rows][d] normalised partial outputs
-  float* part_l;   // [ctas][2][rows] their base-2 log-sum-exp
-  int64_t q_stride;
-  int q_heads;
-  int group;
-  int counted;
-  int ctas;
-  int whole;       // units are not divided
-  float scale2;    // softmax scale times log2(e)
-};
-
-struct SeqWork {
-  int64_t first;  // row of its first token
-  int n, base;    // rows; position of the first one
-  int tiles;      // query tiles of a kv head
-  int chunks;     // chunks of a unit
-  int weight;     // its length on the line: its chunks, or 1 where units are not divided
-};
-
-template <int ROWS>
-__device__ __forceinline__ SeqWork seq_work(const AttendArgs& a, int s) {
-  const RowSpan r = row_span(a.bt, s);
-  // a length past the block table is taken as the whole table
-  const int64_t most = (int64_t)a.bt.table_width * a.kv.page_size;
-  const int held = (int)min((int64_t)r.len, min(most, (int64_t)1 << 30));
-  SeqWork w;
-  w.first = r.first;
-  w.n = r.n;
-  w.base = a.counted ? held - r.n : held;
-  w.tiles = (int)(((int64_t)r.n * a.group + ROWS - 1) / ROWS);
-  w.chunks = max(1, (w.base + r.n + kChunk - 1) / kChunk);
-  w.weight = a.whole ? 1 : w.chunks;
-  return w;
-}
-
-// prefix[s] = chunks of all units before sequence s, for s in [0, seqs].
-template <int ROWS, int THREADS>
-__device__ __forceinline__ void plan_prefix(const AttendArgs& a, int64_t* prefix) {
-  __shared__ int64_t sums[THREADS / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int64_t carry = 0;
-  for (int base = 0; base < a.bt.seqs; base += THREADS) {
-    const int s = base + tid;
-    int64_t w = 0;
-    if (s < a.bt.seqs) {
-      const SeqWork q = seq_work<ROWS>(a, s);
-      w = (int64_t)q.tiles * a.kv.kv_heads * q.weight;
-    }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(FULL, w, o);
-      if (lane >= o) w += v;
-    }
-    if (lane == 31) sums[warp] = w;
-    __syncthreads();
-    int64_t before = carry;
-    for (int i = 0; i < THREADS / 32; ++i) {
-      if (i < warp) before += sums[i];
-      carry += sums[i];
-    }
-    if (s < a.bt.seqs) prefix[s + 1] = before + w;
-    __syncthreads();
-  }
-  if (tid == 0) prefix[0] = 0;
-  __syncthreads();
-}
-
-__device__ __forceinline__ int64_t used_ctas(const AttendArgs& a, int64_t total) {
-  const int64_t ctas = a.ctas, most = a.whole ? total : (total + kMinChunks - 1) / kMinChunks;
-  return most < 1 ? 1 : (most < ctas ? most : ctas);
-}
-
-// last s with prefix[s] <= x (x < prefix[seqs]): the sequence that holds chunk x
-__device__ __forceinline__ int find_seq(const int64_t* prefix, int seqs, int64_t x) {
-  int lo = 0, hi = seqs;  // prefix[lo] <= x < prefix[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prefix[mid] <= x) lo = mid; else hi = mid;
-  }
-  return lo;
-}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -132,17 +44,6 @@ __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
-  uint32_t r;
-  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-  return r;
-}
-// {1024 + u0, 1024 + u1} in fp16 -> {u0 - 128, u1 - 128}, exactly
-__device__ __forceinline__ uint32_t unbias(uint32_t x) {
-  uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));
-  return r;
-}
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
@@ -154,15 +55,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
-}
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
   uint4 v;
@@ -199,10 +91,10 @@ paged_attend_kernel(const AttendArgs a) {
   const int Hkv = a.kv.kv_heads, P = a.kv.page_size;
 
   grid_wait();
-  plan_prefix<ROWS, kAttendThreads>(a, prefix);
+  plan_prefix<ROWS, kChunk, kAttendThreads>(a, prefix);
   grid_trigger();
   const int64_t total = prefix[a.bt.seqs];
-  const int64_t ctas = used_ctas(a, total);
+  const int64_t ctas = used_ctas<kMinChunks>(a, total);
   if ((int64_t)blockIdx.x >= ctas) return;
   int64_t pos = (int64_t)blockIdx.x * total / ctas;
   const int64_t end = ((int64_t)blockIdx.x + 1) * total / ctas;
@@ -213,7 +105,7 @@ paged_attend_kernel(const AttendArgs a) {
 
   for (int slot = 0; pos < end; slot = 1) {
     const int s = find_seq(prefix, a.bt.seqs, pos);
-    const SeqWork w = seq_work<ROWS>(a, s);
+    const SeqWork w = seq_work<ROWS, kChunk>(a, s);
     const int64_t rel = pos - prefix[s];
     const int unit = (int)(rel / w.weight), c0 = (int)(rel - (int64_t)unit * w.weight);
     const int c1 = a.whole ? w.chunks : (int)min((int64_t)w.chunks, c0 + (end - pos));
@@ -521,13 +413,13 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const AttendArgs a,
   // The attention's CTAs start this kernel after their own wait, so what came
   // before them (the lengths among it) is complete; their parts are read after
   // the wait here, which every CTA makes.
-  const SeqWork w = seq_work<ROWS>(a, s);
+  const SeqWork w = seq_work<ROWS, kChunk>(a, s);
   const bool live = tile < w.tiles && tile * ROWS + r < w.n * a.group;
   int64_t total = 1, ctas = 1, u0 = 0;
   if (live) {
-    plan_prefix<ROWS, THREADS>(a, prefix);
+    plan_prefix<ROWS, kChunk, THREADS>(a, prefix);
     total = prefix[a.bt.seqs];
-    ctas = used_ctas(a, total);
+    ctas = used_ctas<kMinChunks>(a, total);
     u0 = prefix[s] + ((int64_t)h * w.tiles + tile) * w.weight;
   }
   grid_wait();
@@ -660,6 +552,10 @@ int launch_dim(const AttendArgs& a, int nt, int64_t max_context, cudaStream_t st
   return launch_rows<256, T>(a, nt, max_context, stream);
 }
 
+// Query rows of a kv head from which on the tiles of 128 rows take over.
+constexpr int kPrefillFrom = 33;
+inline bool many_rows(int64_t max_new, int group) { return max_new * group >= kPrefillFrom; }
+
 // tiles of 8 query rows, or 16 where a sequence brings more than 8 for a kv head
 inline int attend_nt(int64_t max_new, int group) { return max_new * group <= 8 ? 1 : 2; }
 
@@ -674,6 +570,10 @@ int tq_paged_attend_workspace_size(const tq_paged_kv* kv, int q_heads, int max_n
   if (st != TQ_OK) return st;
   if (!bytes) return TQ_E_ARG;
   if (q_heads <= 0 || q_heads % kv->kv_heads || max_new_tokens < 0) return TQ_E_SHAPE;
+  if (many_rows(max_new_tokens, q_heads / kv->kv_heads)) {
+    *bytes = prefill_workspace(kv->head_dim);
+    return TQ_OK;
+  }
   const int nt = attend_nt(max_new_tokens, q_heads / kv->kv_heads);
   *bytes = (size_t)attend_ctas(kv->head_dim, nt) * 2 * 8 * nt * (kv->head_dim + 1) * sizeof(float);
   return TQ_OK;
@@ -706,11 +606,12 @@ int tq_paged_attend(const tq_paged_kv* kv, const tq_paged_batch* batch, const vo
   a.group = q_heads / kv->kv_heads;
   a.counted = counted;
   a.scale2 = scale * 1.44269504f;
+  a.part_o = (float*)workspace;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (many_rows(batch->max_new_tokens, a.group)) return launch_prefill(a, q_dtype, max_context, s);
   const int nt = attend_nt(batch->max_new_tokens, a.group);
   a.ctas = attend_ctas(kv->head_dim, nt);
-  a.part_o = (float*)workspace;
   a.part_l = a.part_o + (size_t)a.ctas * 2 * 8 * nt * kv->head_dim;
-  cudaStream_t s = (cudaStream_t)stream;
   return q_dtype == TQ_F16 ? launch_dim<__half>(a, nt, max_context, s) : launch_dim<__nv_bfloat16>(a, nt, max_context, s);
 }
 
