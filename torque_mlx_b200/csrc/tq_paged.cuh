@@ -51,7 +51,7 @@ __device__ __forceinline__ int page_id(const tq_paged_kv& kv, const tq_paged_bat
 inline int check_paged_kv(const tq_paged_kv* kv) {
   if (!kv) return TQ_E_ARG;
   if (!valid_head_dim(kv->head_dim)) return TQ_E_HEAD_DIM;
-  if (!valid_page_size(kv->page_size) || kv->kv_heads <= 0 || kv->num_pages < 0 || kv->num_pages > INT32_MAX)
+  if (!valid_page_size(kv->page_size) || kv->kv_heads <= 0 || kv->num_pages <= 0 || kv->num_pages > INT32_MAX)
     return TQ_E_SHAPE;
   if (!kv->k_pages || !kv->v_pages || !kv->k_scales || !kv->v_scales) return TQ_E_ARG;
   if ((uintptr_t)kv->k_pages % 16 || (uintptr_t)kv->v_pages % 16) return TQ_E_SHAPE;

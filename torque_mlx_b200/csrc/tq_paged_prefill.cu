@@ -9,22 +9,24 @@
 //
 // Bound: the two products, 4 d flops for each visible (row, token) pair, on
 // the tensor cores, and the exponentials, which take as long at d = 128 (16 a
-// clock for each SM).  Both tiles are 128 x 128: S = Q K^T and O += P V by
-// tcgen05.mma with fp16 operands and fp32 accumulators in tensor memory; P
-// goes back to tensor memory over S, which it replaces.  K and V tiles are
-// converted from codes to fp16 once for 128 rows.
+// clock for each SM).  S = Q K^T and O += P V run on tcgen05.mma with fp16
+// operands and fp32 accumulators in tensor memory, 128 rows by 64 tokens a
+// step; P goes back to tensor memory over S, which it replaces.  K and V are
+// converted from codes to fp16 in shared memory, 128 tokens at a time, once for
+// all rows of the CTA.
 //
 // A CTA takes 256 rows (128 at d = 256, where tensor memory holds no more):
 // for each 128 of them four softmax warps (a thread a row, no shuffles), four
-// warps that convert the next tiles meanwhile, once for all rows, and one that
-// issues the products.  The two halves take turns: while one's scores are in
-// the softmax, the other's products run.
+// warps that convert the next tiles meanwhile, one that looks up the pages and
+// scales of the tiles to come, and one for each half that issues its products.  Each half has two score buffers, so the next step's scores are
+// ready when a softmax ends, whatever the other half does.
 #include "tq_paged_attend.cuh"
 
 namespace tq {
 
 constexpr int kRows = 128;          // query rows of a product
 constexpr int kTokens = 128;        // tokens of a tile
+constexpr int kStep = 64;           // tokens of a step
 constexpr int kPrefillShare = 2;    // smallest share of a CTA, in tiles
 
 // ---- mbarriers, tensor memory and products ----
@@ -51,8 +53,18 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(FULL, bar_wait(bar, parity)); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// by the one lane that `lead` picks, of a warp that runs this together
+__device__ __forceinline__ void tc_commit(uint32_t bar, uint32_t lead) {
+  asm volatile(
+      "{\n .reg .pred q;\n setp.ne.u32 q, %1, 0;\n"
+      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar),
+      "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t elect() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(r));
+  return r;
 }
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -63,21 +75,25 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
   return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
          (uint64_t)2 << 61;
 }
+// the operand `bytes` further on (shared memory ends below the field's range)
+__device__ __forceinline__ uint64_t further(uint64_t o, uint32_t bytes) { return o + (bytes >> 4); }
 // fp16 operands, fp32 accumulator, M = 128; the second operand's rows are k
 // (columns contiguous) where `by_rows`
 __host__ __device__ constexpr uint32_t shape(int n, bool by_rows) {
   return 1u << 4 | (by_rows ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(kRows >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, uint32_t lead) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add, uint32_t lead) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %4, 0;\n setp.ne.u32 q, %5, 0;\n"
+      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add), "r"(lead)
       : "memory");
 }
 // 32 columns of the thread's lane
@@ -92,6 +108,24 @@ __device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(at)
       : "memory");
+}
+// 64 columns of the thread's lane
+__device__ __forceinline__ void tmem_load64(uint32_t at, float (&v)[64]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[16 * b]), "=r"(r[16 * b + 1]), "=r"(r[16 * b + 2]), "=r"(r[16 * b + 3]), "=r"(r[16 * b + 4]),
+          "=r"(r[16 * b + 5]), "=r"(r[16 * b + 6]), "=r"(r[16 * b + 7]), "=r"(r[16 * b + 8]), "=r"(r[16 * b + 9]),
+          "=r"(r[16 * b + 10]), "=r"(r[16 * b + 11]), "=r"(r[16 * b + 12]), "=r"(r[16 * b + 13]), "=r"(r[16 * b + 14]),
+          "=r"(r[16 * b + 15])
+        : "r"(at + 16 * b)
+        : "memory");
+  // the wait names the registers, so that no use of them moves before it
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int k = 0; k < 64; ++k) asm volatile("" : "+r"(r[k]));
 }
 __device__ __forceinline__ void tmem_store32(uint32_t at, const float (&v)[32]) {
   const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
@@ -139,76 +173,156 @@ template <int D> struct PrefillShape {
   static constexpr int kHalves = D == 256 ? 1 : 2;
   static constexpr int kUnit = kHalves * kRows;            // query rows of a unit
   static constexpr int kStages = D == 256 ? 1 : 2;         // K and V tiles that are held
-  static constexpr int kSoftmax = kHalves * 128;           // threads: softmax, then those that convert, then a warp
+  static constexpr int kSoftmax = kHalves * 128;           // threads: softmax, then those that convert, then two warps
   static constexpr int kConvert = D == 256 ? 256 : 128;
-  static constexpr int kThreads = kSoftmax + kConvert + 32;
+  static constexpr int kThreads = 512;                     // four warpgroups, not all warps of the last one working
+  static constexpr int kWorking = kSoftmax + kConvert + 32 + kHalves * 32;
+  // Registers of a thread, of 128 at launch: softmax, conversion, the rest.
+  static constexpr int kRegsSoftmax = 152, kRegsConvert = 136, kRegsRest = 72;
+  static_assert(kHalves * kRegsSoftmax + kConvert / 128 * kRegsConvert + kRegsRest <= 4 * 128, "more than the launch's");
   static constexpr int kOperand = D / 64 * 128 * 128;      // bytes of 128 rows of Q, K or V in fp16
   static constexpr int kSmem = (kHalves + 2 * kStages) * kOperand + 1024;  // from a 1024-byte boundary on
   static constexpr int kColumns = 512;                     // tensor memory of a half: S (P over it), then O
   static constexpr int kRow = D / 16;                      // pieces of 16 codes of a token
   static constexpr int kPieces = 128 * kRow / kConvert;    // a thread's share of a tile
   static constexpr int kTurn = kConvert / kRow;            // tokens from one piece of a thread to its next
-  static constexpr int kAges = 4;                          // tiles whose page scales are kept
+  static constexpr int kAges = 4;                          // tiles whose pages and scales are kept
 };
 
 // byte offset of elements [8 q, 8 q + 8) of row t within an operand
 __device__ __forceinline__ uint32_t place(int t, int q) { return (uint32_t)((q >> 3) * 16384 + t * 128 + (((q & 7) ^ (t & 7)) << 4)); }
 
-// One half's softmax of a tile: weights of the thread's row to tensor memory.
-// lv and inv are of the tile's chunks of sixteen tokens; columns past `seen`
-// are hidden where MASKED.
-template <bool MASKED>
-__device__ __forceinline__ void weigh(uint32_t at, const float* ks, const float* lv, const float* inv, float kf, float m2,
-                                      int seen, float& l) {
-#pragma unroll 1
-  for (int b = 0; b < 4; ++b) {
-    float v[32];
-    tmem_load32(at + b * 32, v);
-    uint32_t p[16];
+// A step's chunks of sixteen tokens as the softmax uses them: scores times f
+// plus the logarithm of v's scale are the exponents, weights times inv count
+// in the softmax's own sum.  Without a page f is 0 and the exponent -inf.
+struct StepScales {
+  float f[4], lv[4], inv[4];
+
+  __device__ __forceinline__ StepScales(const float* ks, const float* lvs, const float* invs, float kf) {
+    const float4 k = *reinterpret_cast<const float4*>(ks), v = *reinterpret_cast<const float4*>(lvs),
+                 i = *reinterpret_cast<const float4*>(invs);
+    f[0] = k.x, f[1] = k.y, f[2] = k.z, f[3] = k.w;
+    lv[0] = v.x, lv[1] = v.y, lv[2] = v.z, lv[3] = v.w;
+    inv[0] = i.x, inv[1] = i.y, inv[2] = i.z, inv[3] = i.w;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int chunk = 2 * b + u;
-      const bool here = ks[chunk] >= 0.f || ks[chunk] != ks[chunk];
-      const float f = here ? ks[chunk] * kf : 0.f, g = here ? lv[chunk] - m2 : -INFINITY;  // no page: weights of zero
-      const uint64_t ff = pair(f, f), gg = pair(g, g);
-      uint64_t sum = 0;
-#pragma unroll
-      for (int k = 0; k < 16; k += 2) {
-        const float2 s = halves(fma2(pair(v[u * 16 + k], v[u * 16 + k + 1]), ff, gg));
-        float x = ex2(s.x), y = ex2(s.y);
-        if (MASKED) {
-          x = chunk * 16 + k <= seen ? x : 0.f;
-          y = chunk * 16 + k + 1 <= seen ? y : 0.f;
-        }
-        sum = add2(sum, pair(x, y));
-        p[u * 8 + k / 2] = half2_bits(x, y);
-      }
-      const float2 s = halves(sum);
-      l = fmaf(s.x + s.y, inv[chunk], l);
+    for (int c = 0; c < 4; ++c) {
+      const bool none = f[c] < 0.f;
+      f[c] = none ? 0.f : f[c] * kf;
+      lv[c] = none ? -INFINITY : lv[c];
     }
-    tmem_store16(at + b * 16, p);
   }
+};
+
+// The largest exponent of a row's step; columns past `seen` are hidden where
+// MASKED.
+template <bool MASKED>
+__device__ __forceinline__ float highest(const float (&v)[kStep], const StepScales& w, int seen) {
+  float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (!MASKED || c * 16 + k <= seen) x[c] = fmaxf(x[c], v[c * 16 + k]);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) x[c] = fmaf(x[c], w.f[c], w.lv[c]);
+  return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));  // a NaN (nothing visible, or no page) is passed over
 }
 
-// The largest exponent of the thread's row in a tile.
+// The row's weights to tensor memory, and their sum without v's scales to l.
 template <bool MASKED>
-__device__ __forceinline__ float highest(uint32_t at, const float* ks, const float* lv, float kf, int seen) {
-  float top = -INFINITY;
-#pragma unroll 1
-  for (int b = 0; b < 4; ++b) {
-    float v[32];
-    tmem_load32(at + b * 32, v);
+__device__ __forceinline__ void weigh(uint32_t at, const float (&v)[kStep], const StepScales& w, float m2, int seen,
+                                      float& l) {
+  float sums[4];
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    uint64_t s[2][8];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int chunk = 2 * b + u;
-      float x = -INFINITY;
+      const int c = 2 * b + u;
+      const float g = w.lv[c] - m2;
+      const uint64_t ff = pair(w.f[c], w.f[c]), gg = pair(g, g);
 #pragma unroll
-      for (int k = 0; k < 16; ++k)
-        if (!MASKED || chunk * 16 + k <= seen) x = fmaxf(x, v[u * 16 + k]);
-      if (ks[chunk] >= 0.f) top = fmaxf(top, fmaf(x, ks[chunk] * kf, lv[chunk]));
+      for (int k = 0; k < 8; ++k) s[u][k] = fma2(pair(v[c * 16 + 2 * k], v[c * 16 + 2 * k + 1]), ff, gg);
+    }
+    uint32_t p[16];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float2 e = halves(s[u][k]);
+        float x = ex2(e.x), y = ex2(e.y);
+        if (MASKED) {
+          const int col = (2 * b + u) * 16 + 2 * k;
+          x = col <= seen ? x : 0.f;
+          y = col + 1 <= seen ? y : 0.f;
+        }
+        p[u * 8 + k] = half2_bits(x, y);
+        s[u][k] = pair(x, y);
+      }
+    tmem_store16(at + b * 16, p);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int o = 4; o; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < o; ++k) s[u][k] = add2(s[u][k], s[u][k + o]);
+      const float2 e = halves(s[u][0]);
+      sums[2 * b + u] = e.x + e.y;
     }
   }
-  return top;
+  l += fmaf(sums[0], w.inv[0], sums[1] * w.inv[1]) + fmaf(sums[2], w.inv[2], sums[3] * w.inv[3]);
+}
+
+// A part of a unit that falls to a CTA.
+struct Unit {
+  int64_t first;       // row of the sequence's first token
+  int s, h, base, r0;  // sequence, kv head, position of its first row, first row of the unit
+  int nr, last;        // rows; last position that any of them attends
+  int c0, n;           // first tile, tiles
+  int live_halves, slot;
+  bool whole;          // all of the unit's tiles
+};
+
+// The CTA's share of the line of tiles, unit by unit.
+template <int UNIT> struct UnitLine {
+  const AttendArgs& a;
+  const int64_t* prefix;
+  int64_t pos, end;
+  int slot = 0;
+
+  __device__ __forceinline__ UnitLine(const AttendArgs& args, const int64_t* p, int64_t total, int64_t ctas)
+      : a(args), prefix(p), pos((int64_t)blockIdx.x * total / ctas), end(((int64_t)blockIdx.x + 1) * total / ctas) {}
+
+  __device__ __forceinline__ bool next(Unit& u) {
+    if (pos >= end) return false;
+    u.s = find_seq(prefix, a.bt.seqs, pos);
+    const SeqWork w = seq_work<UNIT, kTokens>(a, u.s);
+    const int64_t rel = pos - prefix[u.s];
+    const int unit = (int)(rel / w.weight);
+    u.c0 = (int)(rel - (int64_t)unit * w.weight);
+    const int c1 = a.whole ? w.chunks : (int)min((int64_t)w.chunks, u.c0 + (end - pos));
+    u.h = unit / w.tiles;
+    u.r0 = (unit - u.h * w.tiles) * UNIT;
+    u.nr = min(UNIT, w.n * a.group - u.r0);
+    u.first = w.first;
+    u.base = w.base;
+    u.last = w.base + (u.r0 + u.nr - 1) / a.group;
+    u.n = u.last < 0 ? 0 : max(0, min(c1, u.last / kTokens + 1) - u.c0);
+    u.live_halves = u.nr > kRows ? 2 : 1;
+    u.whole = u.c0 == 0 && c1 == w.chunks;
+    u.slot = slot;
+    slot = 1;
+    pos += a.whole ? 1 : c1 - u.c0;
+    return true;
+  }
+};
+
+// a barrier of the working warps, wherever they call it
+template <int THREADS> __device__ __forceinline__ void meet() { asm volatile("barrier.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+template <int THREADS> __device__ __forceinline__ void meet_issuers() { asm volatile("barrier.sync 2, %0;" ::"n"(THREADS) : "memory"); }
+template <int REGS, bool MORE> __device__ __forceinline__ void set_registers() {
+  if (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
 template <int D, typename T>
@@ -216,10 +330,13 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   using Shape = PrefillShape<D>;
   constexpr int H = Shape::kHalves, ST = Shape::kStages, UNIT = Shape::kUnit;
   extern __shared__ __align__(1024) uint8_t prefill_smem[];
-  __shared__ uint64_t bars[4 * ST + 3 * H];
+  __shared__ uint64_t bars[4 * ST + 6 * H + 2 * Shape::kAges];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int failed;
-  __shared__ float page_k[Shape::kAges][8], page_lv[Shape::kAges][8], page_inv[Shape::kAges][8];
+  // of a tile's chunks of sixteen tokens: page and head (0 and a k scale of -1
+  // where there is no page), scales, and whether v is left out of the product
+  __shared__ uint32_t page_at[Shape::kAges][8], page_drop[Shape::kAges];
+  __shared__ __align__(16) float page_k[Shape::kAges][8], page_lv[Shape::kAges][8], page_inv[Shape::kAges][8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t raw = (uint32_t)__cvta_generic_to_shared(prefill_smem), base = (raw + 1023u) & ~1023u;
   uint8_t* const smem = prefill_smem + (base - raw);
@@ -228,7 +345,8 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   int64_t* prefix = reinterpret_cast<int64_t*>(sv + ST * Shape::kOperand);
   const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
   const uint32_t k_full = bar0, k_empty = k_full + 8 * ST, v_full = k_empty + 8 * ST, v_empty = v_full + 8 * ST;  // [stage]
-  const uint32_t s_done = v_empty + 8 * ST, p_full = s_done + 8 * H, pv_done = p_full + 8 * H;                     // [half]
+  const uint32_t s_done = v_empty + 8 * ST, p_full = s_done + 16 * H, pv_done = p_full + 16 * H;  // [half][buffer]
+  const uint32_t page_full = pv_done + 16 * H, page_empty = page_full + 8 * Shape::kAges;  // [age]
 
   grid_wait();
   plan_prefix<UNIT, kTokens, Shape::kThreads>(a, prefix);
@@ -240,18 +358,22 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
     for (int i = 0; i < ST; ++i) {
       bar_init(k_full + 8 * i, Shape::kConvert);
       bar_init(v_full + 8 * i, Shape::kConvert);
-      bar_init(k_empty + 8 * i, 1);
-      bar_init(v_empty + 8 * i, 1);
+      bar_init(k_empty + 8 * i, H);
+      bar_init(v_empty + 8 * i, H);
     }
-    for (int i = 0; i < H; ++i) {
+    for (int i = 0; i < 2 * H; ++i) {
       bar_init(s_done + 8 * i, 1);
       bar_init(p_full + 8 * i, 128);
       bar_init(pv_done + 8 * i, 1);
     }
+    for (int i = 0; i < Shape::kAges; ++i) {
+      bar_init(page_full + 8 * i, 32);
+      bar_init(page_empty + 8 * i, H);
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
   }
-  constexpr int kIssuer = Shape::kThreads / 32 - 1;  // the warp of the products
+  constexpr int kIssuer = Shape::kWorking / 32 - H;  // the warps of the products: one for each half
   if (warp == kIssuer) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      (uint32_t)__cvta_generic_to_shared(&tmem_at)),
@@ -262,140 +384,173 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_at;  // half i: S at 256 i, O at 256 i + 128
+  const uint32_t tmem = tmem_at;  // half i: S buffers at 256 i and 256 i + 64, O at 256 i + 128
 
   const int Hkv = a.kv.kv_heads, P = a.kv.page_size;
-  int64_t pos = (int64_t)blockIdx.x * total / ctas;
-  const int64_t end = ((int64_t)blockIdx.x + 1) * total / ctas;
-  uint32_t tiles_done = 0, half_done[2] = {0, 0};  // of the units before: the barriers' phases
-  for (int slot = 0; pos < end; slot = 1) {
-    const int s = find_seq(prefix, a.bt.seqs, pos);
-    const SeqWork w = seq_work<UNIT, kTokens>(a, s);
-    const int64_t rel = pos - prefix[s];
-    const int unit = (int)(rel / w.weight), c0 = (int)(rel - (int64_t)unit * w.weight);
-    const int c1 = a.whole ? w.chunks : (int)min((int64_t)w.chunks, c0 + (end - pos));
-    const int h = unit / w.tiles, r0 = (unit - h * w.tiles) * UNIT;
-    const int nr = min(UNIT, w.n * a.group - r0);
-    const int last = w.base + (r0 + nr - 1) / a.group;  // last position that a row attends
-    const int n = last < 0 ? 0 : max(0, min(c1, last / kTokens + 1) - c0);
-    const int live_halves = H == 2 && nr > kRows ? 2 : 1;
-    pos += a.whole ? 1 : c1 - c0;
-
-    const int half = H == 2 ? (tid >> 7) & 1 : 0;  // softmax threads
-    float kf = 0.f;                                // the row's score factor
-    int limit = -1, free_to = 0;
-    if (tid < Shape::kSoftmax) {
-      // ---- the row's query, times a power of two that makes fp16 hold it, to shared memory ----
-      const int r = r0 + tid;
-      const bool live = tid < nr;
-      const T* row = reinterpret_cast<const T*>(a.q) + (w.first + r / a.group) * a.q_stride +
-                     (int64_t)(h * a.group + r % a.group) * D;
-      uint8_t* sq = smem + half * Shape::kOperand;
-      float up = a.scale2 < 0.f ? -1.f : 1.f, down = 1.f;
-      if (!Exact<T>::fp16) {
-        float top = 0.f;
-        if (live) {
+  // Each role walks the CTA's units by itself; all meet at the start and at the
+  // end of a unit.
+  uint32_t tiles_done = 0;         // of the units before: the barriers' phases
+  uint32_t half_done[2] = {0, 0};  // step pairs of each half
+  if (tid < Shape::kSoftmax) {
+    set_registers<Shape::kRegsSoftmax, true>();
+    // ---- softmax: a row a thread ----
+    const int half = H == 2 ? tid >> 7 : 0;
+    UnitLine<UNIT> line(a, prefix, total, ctas);
+    for (Unit u; line.next(u);) {
+      const int n = u.n, steps = 2 * n, live_halves = u.live_halves;  // even: each buffer's phases stay in step
+      float kf = 0.f;  // the row's score factor
+      int limit = -1, free_to = 0;
+      {
+        // ---- the row's query, times a power of two that makes fp16 hold it, to shared memory ----
+        const int r = u.r0 + tid;
+        const bool live = tid < u.nr;
+        const T* row = reinterpret_cast<const T*>(a.q) + (u.first + r / a.group) * a.q_stride +
+                       (int64_t)(u.h * a.group + r % a.group) * D;
+        uint8_t* sq = smem + half * Shape::kOperand;
+        float up = a.scale2 < 0.f ? -1.f : 1.f, down = 1.f;
+        if (!Exact<T>::fp16) {
+          float top = 0.f;
+          if (live) {
 #pragma unroll 4
-          for (int q = 0; q < D / 8; ++q) {
-            float f[8];
-            load8(row + 8 * q, f);
+            for (int q = 0; q < D / 8; ++q) {
+              float f[8];
+              load8(row + 8 * q, f);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (fabsf(f[k]) <= 3.402823466e38f) top = fmaxf(top, fabsf(f[k]));
+              for (int k = 0; k < 8; ++k)
+                if (fabsf(f[k]) <= 3.402823466e38f) top = fmaxf(top, fabsf(f[k]));
+            }
           }
+          int e = top > 0.f ? 13 - (ilogbf(top) + 1) : 0;
+          e = min(120, max(-120, e));
+          up *= __int_as_float((e + 127) << 23);
+          down = __int_as_float((127 - e) << 23);
         }
-        int e = top > 0.f ? 13 - (ilogbf(top) + 1) : 0;
-        e = min(120, max(-120, e));
-        up *= __int_as_float((e + 127) << 23);
-        down = __int_as_float((127 - e) << 23);
-      }
 #pragma unroll 4
-      for (int q = 0; q < D / 8; ++q) {
-        float f[8] = {};
-        if (live) load8(row + 8 * q, f);
-        uint4 v;
-        v.x = half2_bits(f[0] * up, f[1] * up);
-        v.y = half2_bits(f[2] * up, f[3] * up);
-        v.z = half2_bits(f[4] * up, f[5] * up);
-        v.w = half2_bits(f[6] * up, f[7] * up);
-        *reinterpret_cast<uint4*>(sq + place(tid & 127, q)) = v;
+        for (int q = 0; q < D / 8; ++q) {
+          float f[8] = {};
+          if (live) load8(row + 8 * q, f);
+          uint4 v;
+          v.x = half2_bits(f[0] * up, f[1] * up);
+          v.y = half2_bits(f[2] * up, f[3] * up);
+          v.z = half2_bits(f[4] * up, f[5] * up);
+          v.w = half2_bits(f[6] * up, f[7] * up);
+          *reinterpret_cast<uint4*>(sq + place(tid & 127, q)) = v;
+        }
+        kf = fabsf(a.scale2) * down;
+        limit = u.base + r / a.group;
+        free_to = u.base + (u.r0 + half * kRows) / a.group;  // positions up to here need no mask
+        proxy_fence();
       }
-      kf = fabsf(a.scale2) * down;
-      limit = w.base + r / a.group;
-      free_to = w.base + (r0 + half * kRows) / a.group;  // positions up to here need no mask
-      proxy_fence();
-    }
-    __syncthreads();  // Q is complete; the last unit's accumulators have been read
-    bool ok = true;
-    float m2 = kNoScore, l = 0.f;
-
-    if (tid < Shape::kSoftmax) {
-      // ---- softmax: a row a thread ----
-      const uint32_t t_s = tmem + half * 256 + ((uint32_t)((warp & 3) * 32) << 16), t_o = t_s + 128;
-      for (int i = 0; i < n && half < live_halves; ++i) {
-        const uint32_t ph = (half_done[half] + i) & 1, age = (tiles_done + i) % Shape::kAges;
-        if (!(ok = warp_wait(s_done + 8 * half, ph))) break;
-        tc_fence_after();
-        const int tok = (c0 + i) * kTokens;
-        const bool masked = tok + kTokens - 1 > free_to;
-        const int seen = limit - tok;  // columns 0..seen are visible
-        const float *ks = page_k[age], *lv = page_lv[age], *inv = page_inv[age];
-        const float top = masked ? highest<true>(t_s, ks, lv, kf, seen) : highest<false>(t_s, ks, lv, kf, seen);
-        if (__any_sync(FULL, top > m2 + kLazy)) {
-          const float nm = fmaxf(m2, top), f = ex2(m2 - nm);
-          m2 = nm;
-          l *= f;
-          if (i > 0) {  // the sums of the tiles before: their products are complete
+      meet<Shape::kWorking>();  // Q is complete
+      bool ok = true;
+      float m2 = kNoScore, l = 0.f;
+      {
+        const uint32_t t_half = tmem + half * 256 + ((uint32_t)((warp & 3) * 32) << 16), t_o = t_half + 128;
+        for (int j = 0; j < steps && half < live_halves; ++j) {
+          const uint32_t buf = j & 1, ph = (half_done[half] + (j >> 1)) & 1, age = (tiles_done + (j >> 1)) % Shape::kAges;
+          if (!(ok = warp_wait(s_done + 8 * (2 * half + buf), ph))) break;
+          tc_fence_after();
+          const StepScales scales(page_k[age] + 4 * buf, page_lv[age] + 4 * buf, page_inv[age] + 4 * buf, kf);
+          float v[kStep];
+          tmem_load64(t_half + buf * kStep, v);
+          const int tok = u.c0 * kTokens + j * kStep;
+          const bool masked = tok + kStep - 1 > free_to;
+          const int seen = limit - tok;  // columns 0..seen are visible
+          const float top = masked ? highest<true>(v, scales, seen) : highest<false>(v, scales, seen);
+          if (__any_sync(FULL, top > m2 + kLazy)) {
+            const float nm = fmaxf(m2, top), f = ex2(m2 - nm);
+            m2 = nm;
+            l *= f;
+            if (j > 0) {  // the sums of the steps before, once their products are complete
+              if (!(ok = warp_wait(pv_done + 8 * (2 * half + 1 - buf), (half_done[half] + ((j - 1) >> 1)) & 1))) break;
+              tc_fence_after();
 #pragma unroll 1
-            for (int b = 0; b < D / 32; ++b) {
-              float v[32];
-              tmem_load32(t_o + b * 32, v);
+              for (int b = 0; b < D / 16; ++b) {
+                uint32_t x[16];
+                asm volatile(
+                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                    "\n\ttcgen05.wait::ld.sync.aligned;"
+                    : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]),
+                      "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+                    : "r"(t_o + b * 16)
+                    : "memory");
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[k] *= f;
-              tmem_store32(t_o + b * 32, v);
+                for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
+                tmem_store16(t_o + b * 16, x);
+              }
+            }
+          }
+          if (masked) weigh<true>(t_half + buf * kStep, v, scales, m2, seen, l);
+          else weigh<false>(t_half + buf * kStep, v, scales, m2, seen, l);
+          tmem_store_wait();
+          tc_fence_before();
+          bar_arrive(p_full + 8 * (2 * half + buf));
+        }
+      }
+      if (!ok) failed = 1;
+      tiles_done += n;
+      half_done[0] += n;
+      if (live_halves == 2) half_done[1] += n;
+      {
+        const bool mine = n > 0 && half < live_halves;
+        if (mine && ok && !warp_wait(pv_done + 8 * (2 * half + 1), (half_done[half] - 1) & 1)) failed = 1;
+        tc_fence_after();
+        const bool whole = u.whole;
+        const float inv = failed ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);
+        const float lse = l == 0.f ? -INFINITY : m2 + __log2f(l);
+        const int r = u.r0 + tid;
+        const int64_t row = u.first + r / a.group, hq = u.h * a.group + r % a.group;
+        const int64_t part = ((int64_t)blockIdx.x * 2 + u.slot) * UNIT + tid;
+        const uint32_t t_o = tmem + half * 256 + 128 + ((uint32_t)((warp & 3) * 32) << 16);
+#pragma unroll 1
+        for (int b = 0; b < D / 32 && half < live_halves; ++b) {
+          float v[32];
+          if (mine) tmem_load32(t_o + b * 32, v);
+          if (tid < u.nr) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              float f[8];
+#pragma unroll
+              for (int x = 0; x < 8; ++x) f[x] = mine ? v[k + x] * inv : 0.f;
+              if (whole) store8(reinterpret_cast<T*>(a.out) + (row * a.q_heads + hq) * D + b * 32 + k, f);
+              else store8(a.part_o + part * D + b * 32 + k, f);
             }
           }
         }
-        if (masked) weigh<true>(t_s, ks, lv, inv, kf, m2, seen, l);
-        else weigh<false>(t_s, ks, lv, inv, kf, m2, seen, l);
-        tmem_store_wait();
-        tc_fence_before();
-        bar_arrive(p_full + 8 * half);
+        if (tid < u.nr) {
+          if (!whole) a.part_l[part] = lse;
+          else if (a.lse) a.lse[row * a.q_heads + hq] = lse * 0.69314718f;
+        }
       }
-    } else if (warp != kIssuer) {
-      // ---- conversion of the tiles' codes ----
+      tc_fence_before();
+      meet<Shape::kWorking>();  // the accumulators have been read
+      tc_fence_after();
+      if (failed) break;  // the phases are not in step any more
+    }
+  } else if (tid < Shape::kSoftmax + Shape::kConvert) {
+    set_registers<Shape::kRegsConvert, true>();
+    // ---- conversion of the tiles' codes ----
+    UnitLine<UNIT> line(a, prefix, total, ctas);
+    for (Unit u; line.next(u);) {
+      const int n = u.n;
+      meet<Shape::kWorking>();
+      bool ok = true;
       constexpr int PIECES = Shape::kPieces, TURN = Shape::kTurn;
       const int pt = tid - Shape::kSoftmax, t0 = pt / Shape::kRow, q = pt % Shape::kRow;
       // Lanes of the odd blocks of 64 elements start with the second half of
       // their sixteen, so that eight lanes fill eight columns.
       const int turn = (q >> 2) & 1;
       const uint32_t to_a = place(t0, 2 * q + turn), to_b = place(t0, 2 * q + 1 - turn);
-      uint4 kr[PIECES], vr[PIECES];  // codes of the next tile
-      float most = -INFINITY;        // log2 of the largest v scale so far
-      // lanes 0..7: pages of the chunks of the tile that is loaded next, and the
-      // scales of that and of the one that is stored next
-      int ids = -1, ids_now = -1;
-      float scale_k = 0.f, scale_v = 0.f, scale_k_now = 0.f, scale_v_now = 0.f;
-      auto fetch_ids = [&](int i) {
-        const int tok = (c0 + i) * kTokens + lane * 16;
-        ids = lane < 8 && i < n && tok <= last ? page_id(a.kv, a.bt, s, tok / P) : -1;
-      };
-      auto fetch_scales = [&]() {
-        if (ids >= 0) {
-          scale_k = a.kv.k_scales[(int64_t)ids * Hkv + h];
-          scale_v = a.kv.v_scales[(int64_t)ids * Hkv + h];
-        }
-      };
-      auto load = [&](const uint8_t* pages, int i, uint4 (&reg)[PIECES]) {
-        const int in_page = (c0 + i) * kTokens + t0;
+      const uint32_t page_bytes = (uint32_t)P * D;  // of a head
+      uint4 kr[PIECES], vr[PIECES];                 // codes of the next tile
+      // A tile starts at a page boundary, so a piece's place in its page is the
+      // same in every tile.
+      auto load = [&](const uint8_t* pages, uint32_t age, uint4 (&reg)[PIECES]) {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-          const int id = __shfl_sync(FULL, ids, (t0 + TURN * j) >> 4);
-          reg[j] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-          if (id >= 0) {
-            const int64_t row = ((int64_t)id * Hkv + h) * P + ((in_page + TURN * j) & (P - 1));
-            reg[j] = *reinterpret_cast<const uint4*>(pages + row * D + q * 16);
-          }
+          const int tok = t0 + TURN * j;
+          const uint8_t* block = pages + (uint64_t)page_at[age][tok >> 4] * page_bytes;
+          reg[j] = *reinterpret_cast<const uint4*>(block + ((tok & (P - 1)) * D + q * 16));
         }
       };
       auto store = [&](uint8_t* to, const uint4 (&reg)[PIECES]) {
@@ -413,35 +568,22 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
           *reinterpret_cast<uint4*>(to + to_b + j * (TURN * 128)) = turn ? lo : hi;
         }
       };
-      fetch_ids(0);
-      fetch_scales();
-      load(a.kv.k_pages, 0, kr);
-      load(a.kv.v_pages, 0, vr);
-      for (int i = 0; i < n; ++i) {
+      auto pages_of = [&](uint32_t tile) { return warp_wait(page_full + 8 * (tile % Shape::kAges), (tile / Shape::kAges) & 1); };
+      if (n > 0 && (ok = pages_of(tiles_done))) {
+        load(a.kv.k_pages, tiles_done % Shape::kAges, kr);
+        load(a.kv.v_pages, tiles_done % Shape::kAges, vr);
+      }
+      for (int i = 0; i < n && ok; ++i) {
         const uint32_t tile = tiles_done + i, st = tile % ST, use = tile / ST;
-        ids_now = ids, scale_k_now = scale_k, scale_v_now = scale_v;
-        fetch_ids(i + 1);
+        const uint32_t drop = page_drop[tile % Shape::kAges];
         if (use > 0 && !(ok = warp_wait(k_empty + 8 * st, (use - 1) & 1))) break;
-        // page scales, for the softmax, and chunks whose v is left out
-        const float lv = log2f(scale_v_now);
-        float top = ids_now >= 0 ? lv : -INFINITY;
-#pragma unroll
-        for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
-        most = fmaxf(most, __shfl_sync(FULL, top, 0));
-        const float least = fmaxf(most - 40.f, -90.f);
-        const uint32_t drop = __ballot_sync(FULL, lane < 8 && ids_now >= 0 && lv < least);
-        if (pt < 8) {
-          const uint32_t age = tile % Shape::kAges;
-          const float use_lv = ids_now < 0 ? 0.f : (lv < least ? least : lv);
-          page_k[age][lane] = ids_now >= 0 ? scale_k_now : -1.f;
-          page_lv[age][lane] = use_lv;
-          page_inv[age][lane] = ex2(-use_lv);
-        }
         store(sk + st * Shape::kOperand, kr);
         proxy_fence();
         bar_arrive(k_full + 8 * st);
-        load(a.kv.k_pages, i + 1, kr);
-        fetch_scales();
+        if (i + 1 < n) {
+          if (!(ok = pages_of(tile + 1))) break;
+          load(a.kv.k_pages, (tile + 1) % Shape::kAges, kr);
+        }
         if (drop) {
 #pragma unroll
           for (int j = 0; j < PIECES; ++j)
@@ -451,97 +593,142 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         store(sv + st * Shape::kOperand, vr);
         proxy_fence();
         bar_arrive(v_full + 8 * st);
-        load(a.kv.v_pages, i + 1, vr);
+        if (i + 1 < n) load(a.kv.v_pages, (tile + 1) % Shape::kAges, vr);
       }
-    } else if (lane == 0) {
-      // ---- products: S of the first tile, then P V and the next S of each half in turn ----
-      auto scores = [&](int i, int x) {
-        const uint32_t st = (tiles_done + i) % ST;
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-          mma_ss(tmem + x * 256, operand(base + x * Shape::kOperand + off, 16),
-                 operand(k_at + st * Shape::kOperand + off, 16), shape(kTokens, false), k > 0);
-        }
-        tc_commit(s_done + 8 * x);
-        if (x == live_halves - 1) tc_commit(k_empty + 8 * st);
-      };
-      if (n > 0 && (ok = bar_wait(k_full + 8 * (tiles_done % ST), (tiles_done / ST) & 1))) {
-        tc_fence_after();
-        for (int x = 0; x < live_halves; ++x) scores(0, x);
-      }
-      for (int i = 0; i < n && ok; ++i) {
-        const uint32_t tile = tiles_done + i, st = tile % ST;
-        for (int x = 0; x < live_halves; ++x) {
-          if (x == 0 && !(ok = bar_wait(v_full + 8 * st, (tile / ST) & 1))) break;
-          if (!(ok = bar_wait(p_full + 8 * x, (half_done[x] + i) & 1))) break;
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < kTokens / 16; ++k)
-            mma_ts(tmem + x * 256 + 128, tmem + x * 256 + k * 8, operand(v_at + st * Shape::kOperand + k * 2048, 16384),
-                   shape(D, true), i > 0 || k > 0);
-          tc_commit(pv_done + 8 * x);
-          if (x == live_halves - 1) tc_commit(v_empty + 8 * st);
-          if (i + 1 < n) {
-            if (x == 0) {
-              const uint32_t next = tile + 1;
-              if (!(ok = bar_wait(k_full + 8 * (next % ST), (next / ST) & 1))) break;
-              tc_fence_after();
-            }
-            scores(i + 1, x);
-          }
-        }
-      }
-    }
-    if (!ok) failed = 1;
-    tiles_done += n;
-    half_done[0] += n;
-    if (live_halves == 2) half_done[1] += n;
 
-    // ---- the unit's rows ----
-    if (tid < Shape::kSoftmax) {
-      const bool mine = n > 0 && half < live_halves;
-      if (mine && ok && !warp_wait(pv_done + 8 * half, (half_done[half] - 1) & 1)) failed = 1;
-      tc_fence_after();
-      const bool whole = c0 == 0 && c1 == w.chunks;
-      const float inv = failed ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);
-      const float lse = l == 0.f ? -INFINITY : m2 + __log2f(l);
-      const int r = r0 + tid;
-      const int64_t row = w.first + r / a.group, hq = h * a.group + r % a.group;
-      const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * UNIT + tid;
-      const uint32_t t_o = tmem + half * 256 + 128 + ((uint32_t)((warp & 3) * 32) << 16);
-#pragma unroll 1
-      for (int b = 0; b < D / 32 && half < live_halves; ++b) {
-        float v[32];
-        if (mine) tmem_load32(t_o + b * 32, v);
-        if (tid < nr) {
+      if (!ok) failed = 1;
+      tiles_done += n;
+      meet<Shape::kWorking>();
+      if (failed) break;
+    }
+  } else {
+    set_registers<Shape::kRegsRest, false>();
+    if (warp == kIssuer - 1) {
+      // ---- pages and scales of the tiles, ahead of the conversion ----
+      UnitLine<UNIT> line(a, prefix, total, ctas);
+      for (Unit u; line.next(u);) {
+        const int n = u.n;
+        meet<Shape::kWorking>();
+        bool ok = true;
+        float most = -INFINITY;  // log2 of the largest v scale so far
+        auto find = [&](int i) {
+          const int tok = (u.c0 + i) * kTokens + lane * 16;
+          return lane < 8 && i < n && tok <= u.last ? page_id(a.kv, a.bt, u.s, tok / P) : -1;
+        };
+        int next = find(0);
+        for (int i = 0; i < n; ++i) {
+          const uint32_t tile = tiles_done + i, age = tile % Shape::kAges, use = tile / Shape::kAges;
+          const int id = next;
+          next = find(i + 1);
+          const int64_t block = (int64_t)max(id, 0) * Hkv + u.h;
+          float ks = -1.f, lv = -INFINITY;
+          if (id >= 0) {
+            ks = a.kv.k_scales[block];
+            lv = log2f(a.kv.v_scales[block]);
+          }
+          float top = lv;
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            float f[8];
+          for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
+          most = fmaxf(most, __shfl_sync(FULL, top, 0));
+          const float least = fmaxf(most - 40.f, -90.f);
+          const uint32_t drop = __ballot_sync(FULL, id >= 0 && lv < least);
+          if (use > 0 && !(ok = warp_wait(page_empty + 8 * age, (use - 1) & 1))) break;
+          if (lane < 8) {
+            const float use_lv = id < 0 ? 0.f : (lv < least ? least : lv);
+            page_at[age][lane] = (uint32_t)block;
+            page_k[age][lane] = ks;
+            page_lv[age][lane] = use_lv;
+            page_inv[age][lane] = ex2(-use_lv);
+            if (lane == 0) page_drop[age] = drop;
+          }
+          __syncwarp();
+          bar_arrive(page_full + 8 * age);
+        }
+
+        if (!ok) failed = 1;
+        tiles_done += n;
+        meet<Shape::kWorking>();
+        if (failed) break;
+      }
+    } else if (warp >= kIssuer && warp < kIssuer + H) {
+      // ---- products of a half: S of two steps, then P V of each step and the S after the next ----
+      const int x = warp - kIssuer;
+      const uint32_t lead = elect(), t_s = tmem + x * 256, t_o = t_s + 128;
+      const uint64_t q_op = operand(base + x * Shape::kOperand, 16), k_op = operand(k_at, 16), v_op = operand(v_at, 16384);
+      const uint32_t s_bar = s_done + 16 * x, p_bar = p_full + 16 * x, pv_bar = pv_done + 16 * x;
+      uint32_t pairs_done = 0;  // of this half's steps
+      UnitLine<UNIT> line(a, prefix, total, ctas);
+      for (Unit u; line.next(u);) {
+        const int n = u.n;
+        const bool mine = x < u.live_halves, alone = H == 2 && u.live_halves == 1;
+        meet<Shape::kWorking>();
+        tc_fence_after();
+        bool ok = true;
+        // a tile is given back by both halves; the only one at work arrives for both
+        auto give_back = [&](uint32_t bar) {
+          tc_commit(bar, lead);
+          if (alone) tc_commit(bar, lead);
+        };
+        auto scores = [&](uint32_t st, uint32_t buf) {
+          const uint64_t k = further(k_op, st * Shape::kOperand + buf * (kStep * 128));
 #pragma unroll
-            for (int x = 0; x < 8; ++x) f[x] = mine ? v[k + x] * inv : 0.f;
-            if (whole) store8(reinterpret_cast<T*>(a.out) + (row * a.q_heads + hq) * D + b * 32 + k, f);
-            else store8(a.part_o + part * D + b * 32 + k, f);
+          for (int i = 0; i < D / 16; ++i) {
+            const uint32_t off = (i >> 2) * 16384 + (i & 3) * 32;
+            mma_ss(t_s + buf * kStep, further(q_op, off), further(k, off), shape(kStep, false), i > 0, lead);
+          }
+          tc_commit(s_bar + 8 * buf, lead);
+          if (buf == 1) give_back(k_empty + 8 * st);
+        };
+        auto values = [&](uint32_t st, uint32_t buf, bool add) {
+          const uint64_t v = further(v_op, st * Shape::kOperand + buf * (kStep * 128));
+#pragma unroll
+          for (int k = 0; k < kStep / 16; ++k)
+            mma_ts(t_o, t_s + buf * kStep + k * 8, further(v, k * 2048), shape(D, true), add || k > 0, lead);
+          tc_commit(pv_bar + 8 * buf, lead);
+        };
+        if (mine && n > 0) {
+          uint32_t st = tiles_done % ST;
+          ok = warp_wait(k_full + 8 * st, (tiles_done / ST) & 1);
+          if (ok) {
+            tc_fence_after();
+            scores(st, 0);
+            scores(st, 1);
+          }
+          for (int i = 0; i < n && ok; ++i) {
+            const uint32_t tile = tiles_done + i, next = tile + 1, ph = (pairs_done + i) & 1;
+            st = tile % ST;
+            if (!(ok = warp_wait(v_full + 8 * st, (tile / ST) & 1))) break;
+            if (!(ok = warp_wait(p_bar, ph))) break;
+            tc_fence_after();
+            values(st, 0, i > 0);
+            if (i + 1 < n) {
+              if (!(ok = warp_wait(k_full + 8 * (next % ST), (next / ST) & 1))) break;
+              tc_fence_after();
+              scores(next % ST, 0);
+            }
+            if (!(ok = warp_wait(p_bar + 8, ph))) break;
+            tc_fence_after();
+            values(st, 1, true);
+            give_back(v_empty + 8 * st);
+            give_back(page_empty + 8 * (tile % Shape::kAges));
+            if (i + 1 < n) scores(next % ST, 1);
           }
         }
+        if (!ok) failed = 1;
+        tiles_done += n;
+        if (mine) pairs_done += n;
+        meet<Shape::kWorking>();
+        tc_fence_after();
+        if (failed) break;
       }
-      if (tid < nr) {
-        if (!whole) a.part_l[part] = lse;
-        else if (a.lse) a.lse[row * a.q_heads + hq] = lse * 0.69314718f;
+      if (failed)  // products in flight end before the memory goes back
+        for (int i = 0; i < 2; ++i) bar_wait(pv_bar + 8 * i, 0);
+      meet_issuers<32 * H>();
+      if (x == 0) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Shape::kColumns));
       }
-      tc_fence_before();
     }
-    __syncthreads();
-    tc_fence_after();
-    if (failed) break;  // the phases are not in step any more
-  }
-  if (failed && tid == 0) {  // products in flight end before the memory goes back
-    for (int i = 0; i < H; ++i) bar_wait(pv_done + 8 * i, 0);
-  }
-  __syncthreads();
-  if (warp == kIssuer) {
-    __syncwarp();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)Shape::kColumns));
   }
 }
 
@@ -570,25 +757,33 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const AttendArg
   const int n = last - first + 1;
   const int slot0 = (int64_t)first * total / ctas < u0 ? 1 : 0;
   auto part_of = [&](int i) { return ((int64_t)(first + i) * 2 + (i == 0 ? slot0 : 0)) * UNIT + in_tile; };
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, a.part_l[part_of(i)]);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
-  if (top == -INFINITY) top = 0.f;
   constexpr int E = D / 32;  // elements of a lane: pairs at 2 lane, 64 apart
-  float sum = 0.f, v[E];
+  float top = -INFINITY, sum = 0.f, v[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float f = ex2(a.part_l[part_of(i)] - top);
-    const float2* o = reinterpret_cast<const float2*>(a.part_o + part_of(i) * D) + lane;
-    sum += f;
+  for (int i0 = 0; i0 < n; i0 += 32) {  // a lane holds a part's sum; the parts' rows do not wait for it
+    const float mine = i0 + lane < n ? a.part_l[part_of(i0 + lane)] : -INFINITY;
+    float high = mine;
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 x = o[e * 16];
-      v[e] = fmaf(f, x.x, v[e]);
-      v[e + 1] = fmaf(f, x.y, v[e + 1]);
+    for (int o = 16; o; o >>= 1) high = fmaxf(high, __shfl_xor_sync(FULL, high, o));
+    high = fmaxf(high, top);
+    if (high == -INFINITY) high = 0.f;
+    const float old = ex2(top - high), f = ex2(mine - high);
+    top = high;
+    sum *= old;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] *= old;
+#pragma unroll 4
+    for (int i = i0; i < min(n, i0 + 32); ++i) {
+      const float2* o = reinterpret_cast<const float2*>(a.part_o + part_of(i) * D) + lane;
+      const float fi = __shfl_sync(FULL, f, i - i0);
+      sum += fi;
+#pragma unroll
+      for (int e = 0; e < E; e += 2) {
+        const float2 x = o[e * 16];
+        v[e] = fmaf(fi, x.x, v[e]);
+        v[e + 1] = fmaf(fi, x.y, v[e + 1]);
+      }
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -609,7 +804,7 @@ size_t prefill_workspace(int head_dim) {
 
 template <int D, typename T>
 int launch_prefill_kernel(AttendArgs a, int64_t max_context, cudaStream_t stream) {
-  constexpr int kMostSmem = 227 * 1024 - 1024;
+  constexpr int kMostSmem = 227 * 1024 - 2048;  // the static arrays take the rest
   static bool allowed[kMaxDevices] = {};  // the kernel's attribute is set once for each device
   const int dev = device_index();
   if (!allowed[dev]) {

@@ -108,6 +108,8 @@ class PagedKV8Cache:
                 raise ValueError(f"{name} must be contiguous fp32 [pages, kv_heads]")
             if t.device != key_pages.device:
                 raise ValueError(f"{name} must be on {key_pages.device}")
+        if key_pages.shape[0] == 0 or key_pages.shape[1] == 0:
+            raise ValueError("the pool has no pages or no heads")
         if value_pages.shape != key_pages.shape or value_pages.device != key_pages.device:
             raise ValueError("key_pages and value_pages must match in shape and device")
         validate_head_dim(int(key_pages.shape[3]))
