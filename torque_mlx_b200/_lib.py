@@ -145,12 +145,25 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+BIND_PATH = Path(__file__).resolve().parent / "_torch_bind.so"
+_bind = None
 
 
-def stream_of(index: int) -> int:
-    """Handle of device ``index``'s current CUDA stream."""
-    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+def binding():
+    """The native binding of the serving operators (csrc/tq_torch.cpp), loaded
+    once; demands a CUDA device, like ``load``."""
+    global _bind
+    if _bind is None:
+        load()
+        if not BIND_PATH.exists():
+            raise RuntimeError(f"{BIND_PATH.name} is not built; run `python -m torque_mlx_b200.build`")
+        from importlib.machinery import ExtensionFileLoader
+        from importlib.util import module_from_spec, spec_from_file_location
+        spec = spec_from_file_location("_torch_bind", BIND_PATH, loader=ExtensionFileLoader("_torch_bind", str(BIND_PATH)))
+        module = module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _bind = module
+    return _bind
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

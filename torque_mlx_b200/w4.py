@@ -14,7 +14,6 @@ from ctypes import byref, c_size_t
 import torch
 
 from . import _lib
-from .paged import scratch
 
 GROUP_SIZES = (32, 64, 128)
 _MODES = {"plain": 0, "f32": 1, "rms": 2, "silu": 3}
@@ -26,17 +25,7 @@ class W4Weight:
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, group_size: int):
         self.codes, self.scales = codes, scales
         self.n, self.k, self.group_size = n, k, group_size
-        self.device, self._index = codes.device, codes.get_device()
-        self._need: dict[int, int] = {}  # workspace by token count
-
-    def _workspace(self, tokens: int) -> int:
-        """Bytes of a product's workspace, asked once for each token count."""
-        need = self._need.get(tokens)
-        if need is None:
-            size = c_size_t()
-            _lib.check(_lib.load().tq_gemv_w4_workspace_size(self.n, self.k, tokens, byref(size)), "gemv_w4")
-            need = self._need[tokens] = size.value
-        return need
+        self.device = codes.device
 
     @staticmethod
     def _check_sizes(n: int, k: int, group_size: int) -> tuple[int, int]:
@@ -110,51 +99,8 @@ def gemv_w4(weight: W4Weight, x: torch.Tensor, *, mode: str = "plain", norm_weig
     or the SwiGLU activation of ``[gate | up]`` rows of ``2k`` ("silu").
     Returns ``[tokens, n]`` (or ``[n]``) in x's type (bf16 for "f32").  Made for
     few tokens: the weight is read once for each 32 of them."""
-    lib = _lib.load()
-    if _lib.current_device() != weight._index:
-        with torch.cuda.device(weight.device):
-            return gemv_w4(weight, x, mode=mode, norm_weight=norm_weight, eps=eps, residual=residual, out=out)
-    try:
-        code = _MODES[mode]
-    except KeyError as exc:
-        raise ValueError(f"mode must be one of {sorted(_MODES)}") from exc
-    k, n, dev = weight.k, weight.n, weight.device
-    width = 2 * k if code == 3 else k
-    if x.dim() not in (1, 2) or x.shape[-1] != width or x.get_device() != weight._index:
-        raise ValueError(f"gemv_w4: x must be [tokens, {width}] on {dev}, got {tuple(x.shape)}")
-    dtype = x.dtype
-    if code == 1:
-        if dtype is not torch.float32:
-            raise ValueError(f"gemv_w4: x must be float32 in mode 'f32', got {dtype}")
-        dtype = torch.bfloat16
-    elif dtype is not torch.bfloat16 and not (code == 0 and dtype is torch.float16):
-        raise ValueError(f"gemv_w4: x must be bfloat16{' or float16' if code == 0 else ''} in mode {mode!r}, got {dtype}")
-    tokens = x.shape[0] if x.dim() == 2 else 1
-    if width > 1 and x.stride(-1) != 1:
-        x = x.contiguous()
-    norm = None
-    if code == 2:
-        if (norm_weight is None or norm_weight.dtype != torch.bfloat16 or norm_weight.numel() != k
-                or norm_weight.device != dev or not norm_weight.is_contiguous()):
-            raise ValueError(f"gemv_w4: norm_weight must be contiguous bf16 [{k}] on {dev}")
-        norm = norm_weight.data_ptr()
-    shape = (tokens, n) if x.dim() == 2 else (n,)
-    res = None
-    if residual is not None:
-        if (residual.dtype != dtype or residual.numel() != tokens * n or residual.device != dev
-                or not residual.is_contiguous()):
-            raise ValueError(f"gemv_w4: residual must be contiguous {dtype} {shape} on {dev}")
-        res = residual.data_ptr()
-    if out is None:
-        out = x.new_empty(shape) if dtype is x.dtype else torch.empty(shape, dtype=dtype, device=dev)
-    elif out.dtype != dtype or out.numel() != tokens * n or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"gemv_w4: out must be contiguous {dtype} {shape} on {dev}")
-    need = weight._workspace(tokens)
-    ws = scratch(need, dev).data_ptr() if need else None
-    status = lib.tq_gemv_w4(weight.codes.data_ptr(), weight.scales.data_ptr(), n, k, weight.group_size, x.data_ptr(),
-                            _lib.TQ_F16 if dtype is torch.float16 else _lib.TQ_BF16,
-                            x.stride(0) if x.dim() == 2 else width, code, norm, eps, res, out.data_ptr(), tokens, ws,
-                            need, _lib.stream_of(weight._index))
-    if status:
-        _lib.check(status, "gemv_w4")
-    return out
+    code = _MODES.get(mode)
+    if code is None:
+        raise ValueError(f"mode must be one of {sorted(_MODES)}")
+    return _lib.binding().gemv_w4(weight.codes, weight.scales, weight.n, weight.k, weight.group_size, x, code, norm_weight,
+                                  eps, residual, out)
