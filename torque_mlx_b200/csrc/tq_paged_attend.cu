@@ -320,8 +320,8 @@ paged_attend_kernel(const AttendArgs a) {
           for (int half = 0; half < 2; ++half) {
             const uint32_t sel = half ? 0x7632 : 0x5410;
             const uint32_t x = prmt(v[0][q], v[1][q], sel), y = prmt(v[2][q], v[3][q], sel);
-            const uint32_t a0 = unbias((x & 0x00ff00ffu) | 0x64006400u), a1 = unbias(prmt(x, 0x64646464u, 0x4341));
-            const uint32_t a2 = unbias((y & 0x00ff00ffu) | 0x64006400u), a3 = unbias(prmt(y, 0x64646464u, 0x4341));
+            const uint32_t a0 = unbias(prmt(x, 0x64646464u, 0x4240)), a1 = unbias(prmt(x, 0x64646464u, 0x4341));
+            const uint32_t a2 = unbias(prmt(y, 0x64646464u, 0x4240)), a3 = unbias(prmt(y, 0x64646464u, 0x4341));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma16816(o[(u * VW + q) * 2 + half][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
           }

@@ -63,15 +63,30 @@ template <int BYTES> __device__ __forceinline__ void cp_scales(uint32_t dst, con
 }
 __device__ __forceinline__ void w4_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void w4_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// A constant that stays in a register: a logic operation holds one immediate
+// at most, and two constants folded into it would make two of it.
+__device__ __forceinline__ uint32_t kept(uint32_t c) {
+  asm volatile("" : "+r"(c));
+  return c;
+}
+// (a & mask) | set
+__device__ __forceinline__ uint32_t pick(uint32_t a, uint32_t mask, uint32_t set) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(set));
+  return r;
+}
+
 // eight codes of a word -> A fragment of sixteen rows and columns, code - 8
 template <typename T> struct W4Math;
 template <> struct W4Math<__half> {
-  static __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
+  const uint32_t low = kept(0x000f000fu), high = kept(0x00f000f0u), set = kept(0x64006400u), bias = kept(0x64086408u),
+                 sixteenth = kept(0x2c002c00u), shifted = kept(0xd480d480u);
+  __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) const {
     const uint32_t v = w >> 8;
-    a[0] = sub((w & 0x000f000fu) | 0x64006400u, 0x64086408u);               // 1024 + c - 1032
-    a[1] = sub((v & 0x000f000fu) | 0x64006400u, 0x64086408u);
-    a[2] = fma((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);  // (1024 + 16 c) / 16 - 72
-    a[3] = fma((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
+    a[0] = sub(pick(w, low, set), bias);                 // 1024 + c - 1032
+    a[1] = sub(pick(v, low, set), bias);
+    a[2] = fma(pick(w, high, set), sixteenth, shifted);  // (1024 + 16 c) / 16 - 72
+    a[3] = fma(pick(v, high, set), sixteenth, shifted);
   }
   static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -91,15 +106,16 @@ template <> struct W4Math<__half> {
   }
 };
 template <> struct W4Math<__nv_bfloat16> {
-  static __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) {
-    a[0] = sub((w & 0x000f000fu) | 0x43004300u);  // 128 + c - 136
-    a[2] = sub(((w >> 4) & 0x000f000fu) | 0x43004300u);
-    a[1] = sub(((w >> 8) & 0x000f000fu) | 0x43004300u);
-    a[3] = sub(((w >> 12) & 0x000f000fu) | 0x43004300u);
+  const uint32_t low = kept(0x000f000fu), set = kept(0x43004300u), bias = kept(0x43084308u);
+  __device__ __forceinline__ void expand(uint32_t w, uint32_t (&a)[4]) const {
+    a[0] = sub(pick(w, low, set));  // 128 + c - 136
+    a[2] = sub(pick(w >> 4, low, set));
+    a[1] = sub(pick(w >> 8, low, set));
+    a[3] = sub(pick(w >> 12, low, set));
   }
-  static __device__ __forceinline__ uint32_t sub(uint32_t a) {
+  __device__ __forceinline__ uint32_t sub(uint32_t a) const {
     uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(0x43084308u));
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(bias));
     return r;
   }
   static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -147,7 +163,7 @@ __device__ __forceinline__ void w4_input(const W4Args& a, int64_t m, int64_t k0,
 // NT tiles of eight tokens, SG groups of a block.
 template <int NT, int SG, typename T>
 __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
-  using Math = W4Math<T>;
+  const W4Math<T> math;
   constexpr int UNIT = 1024 + 32 * SG, STAGES = kW4Stages;
   extern __shared__ __align__(128) uint8_t w4_smem[];
   __shared__ float red[kW4Warps][kW4MaxTokens];
@@ -301,12 +317,12 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
             for (int k = 0; k < 4; ++k) sum[nt][k] = 0.f;
         }
         uint32_t f[4];
-        Math::expand(w[2 * i], f);
+        math.expand(w[2 * i], f);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) Math::mma(sum[nt], f, x[nt].x, x[nt].y);
-        Math::expand(w[2 * i + 1], f);
+        for (int nt = 0; nt < NT; ++nt) math.mma(sum[nt], f, x[nt].x, x[nt].y);
+        math.expand(w[2 * i + 1], f);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) Math::mma(sum[nt], f, x[nt].z, x[nt].w);
+        for (int nt = 0; nt < NT; ++nt) math.mma(sum[nt], f, x[nt].z, x[nt].w);
         if ((i + 1) % (4 / SG) == 0) {
           const uint32_t s2 = two[i / (4 / SG)];
           const float s0 = __uint_as_float(s2 << 16), s1 = __uint_as_float(s2 & 0xffff0000u);
