@@ -119,6 +119,22 @@ paged_attend_kernel(const AttendArgs a) {
     const int steps = min(c1, last / kChunk + 1) > c0 + warp && last >= 0
                           ? (min(c1, last / kChunk + 1) - c0 - warp + kAttendWarps - 1) / kAttendWarps
                           : 0;
+    uint4 raw[NT][KI][2];  // the query rows' elements, on their way while the copies are issued
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = r0 + nt * 8 + g;
+      const T* row = reinterpret_cast<const T*>(a.q) + (w.first + r / a.group) * a.q_stride +
+                     (int64_t)(h * a.group + r % a.group) * D;
+#pragma unroll
+      for (int i = 0; i < KI; ++i) {
+        const int piece = D == 64 ? c : 8 * (i >> 1) + 2 * c + (i & 1);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          raw[nt][i][e] = make_uint4(0, 0, 0, 0);
+          if (nt * 8 + g < nr) raw[nt][i][e] = reinterpret_cast<const uint4*>(row + piece * 16)[e];
+        }
+      }
+    }
     auto chunk_page = [&](int it) {
       const int ch = c0 + warp + it * kAttendWarps;
       return it < steps ? page_id(a.kv, a.bt, s, ch * kChunk / P) : -1;
@@ -163,26 +179,15 @@ paged_attend_kernel(const AttendArgs a) {
     int limit[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = r0 + nt * 8 + g;
-      const bool live = nt * 8 + g < nr;
-      const T* row = reinterpret_cast<const T*>(a.q) + (w.first + r / a.group) * a.q_stride +
-                     (int64_t)(h * a.group + r % a.group) * D;
       float x[KI][16];
       float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < KI; ++i) {
-        const int piece = D == 64 ? c : 8 * (i >> 1) + 2 * c + (i & 1);
+      for (int i = 0; i < KI; ++i)
 #pragma unroll
-        for (int e = 0; e < 16; e += 8) {
-          float f[8] = {};
-          if (live) load8(row + piece * 16 + e, f);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            x[i][e + k] = f[k];
-            if (fabsf(f[k]) <= 3.402823466e38f) top = fmaxf(top, fabsf(f[k]));
-          }
+        for (int e = 0; e < 16; ++e) {
+          x[i][e] = to_f32<T>(reinterpret_cast<const T*>(&raw[nt][i][e / 8])[e % 8]);
+          if (fabsf(x[i][e]) <= 3.402823466e38f) top = fmaxf(top, fabsf(x[i][e]));
         }
-      }
       top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
       top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
       int e = 0;  // power of two that takes the largest element to [2^12, 2^13)

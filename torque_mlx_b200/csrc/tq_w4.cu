@@ -235,17 +235,48 @@ __global__ void __launch_bounds__(kW4Threads, 1) w4_kernel(const W4Args a) {
     __syncthreads();
   }
   const int pieces8 = nb * (kW4Block / 8);  // eight columns each
-  for (int i = tid; i < M * pieces8; i += kW4Threads) {
-    const int m = i / pieces8, at = i - m * pieces8;
-    float f[8];
-    w4_input<T>(a, m, k_lo + at * 8, a.mode == kW4Rms ? inv_rms[m] : 0.f, vec, f);
+  auto place = [&](int m, int at) {         // four words, sixteen bytes apart
     const int b = at / 16, j = at % 16 / 2, half = at & 1;
-    uint8_t* dst = xs + ((b * 4 + (j >> 1)) * M + m) * 64 + ((j & 1) * 4 + half * 2) * 2;
+    return xs + ((b * 4 + (j >> 1)) * M + m) * 64 + ((j & 1) * 4 + half * 2) * 2;
+  };
+  auto put = [&](uint8_t* dst, const uint32_t (&w)[4]) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const T lo = from_f32<T>(f[2 * q]), hi = from_f32<T>(f[2 * q + 1]);
-      *reinterpret_cast<uint32_t*>(dst + q * 16) =
-          (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<uint32_t*>(dst + q * 16) = w[q];
+  };
+  if (a.mode == kW4Plain && vec && a.k % 8 == 0) {  // words as they are, four loads of a thread at a time
+    constexpr int U = 4;
+    const int total = M * pieces8, columns8 = (int)(a.k / 8) - (int)(k_lo / 8);
+    for (int i0 = tid; i0 < total; i0 += U * kW4Threads) {
+      uint4 v[U];
+      int m[U], at[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * kW4Threads;
+        m[u] = i / pieces8;
+        at[u] = i - m[u] * pieces8;
+        v[u] = make_uint4(0, 0, 0, 0);
+        if (i < total && at[u] < columns8)
+          v[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.x) + m[u] * a.x_stride + k_lo + at[u] * 8);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * kW4Threads < total) {
+          const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+          put(place(m[u], at[u]), w);
+        }
+    }
+  } else {
+    for (int i = tid; i < M * pieces8; i += kW4Threads) {
+      const int m = i / pieces8, at = i - m * pieces8;
+      float f[8];
+      w4_input<T>(a, m, k_lo + at * 8, a.mode == kW4Rms ? inv_rms[m] : 0.f, vec, f);
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const T lo = from_f32<T>(f[2 * q]), hi = from_f32<T>(f[2 * q + 1]);
+        w[q] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+      }
+      put(place(m, at), w);
     }
   }
   __syncthreads();
