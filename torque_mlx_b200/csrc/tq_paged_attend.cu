@@ -401,8 +401,8 @@ paged_attend_kernel(const AttendArgs a) {
 
 // grid (seqs * kv_heads * tiles, rows, d / DIMS): joins the parts of DIMS
 // elements of one query row.  Few units have many parts each: 256 threads read
-// sixteen of them side by side, 64 elements a CTA.  Many units have two or
-// three: a CTA of 64 threads for a row.
+// sixteen of them side by side, 64 elements a CTA.  More units have a few: a
+// CTA of 64 threads for a row.
 constexpr int kMaxCtas = 148 * 8;
 
 template <int D, int ROWS, int DIMS, int THREADS, typename T>
@@ -538,7 +538,7 @@ int launch_attend(AttendArgs a, int64_t max_context, cudaStream_t stream) {
   if (st != TQ_OK || a.ctas == 1 || a.whole) return st;
   const int64_t rows = (int64_t)a.bt.max_new_tokens * a.group;
   const unsigned y = (unsigned)(rows < 8 * NT ? rows : 8 * NT);
-  if (units * 4 >= a.ctas)
+  if (units * 16 >= a.ctas)
     return launch_dependent(paged_join_kernel<D, 8 * NT, D, 64, T>, dim3((unsigned)units, y), dim3(64), prefix_bytes,
                             stream, a, tiles);
   return launch_dependent(paged_join_kernel<D, 8 * NT, 64, 256, T>, dim3((unsigned)units, y, D / 64), dim3(256),

@@ -178,7 +178,7 @@ template <int D> struct PrefillShape {
   static constexpr int kThreads = 512;                     // four warpgroups, not all warps of the last one working
   static constexpr int kWorking = kSoftmax + kConvert + 32 + kHalves * 32;
   // Registers of a thread, of 128 at launch: softmax, conversion, the rest.
-  static constexpr int kRegsSoftmax = 152, kRegsConvert = 136, kRegsRest = 72;
+  static constexpr int kRegsSoftmax = 168, kRegsConvert = 96, kRegsRest = 72;
   static_assert(kHalves * kRegsSoftmax + kConvert / 128 * kRegsConvert + kRegsRest <= 4 * 128, "more than the launch's");
   static constexpr int kOperand = D / 64 * 128 * 128;      // bytes of 128 rows of Q, K or V in fp16
   static constexpr int kSmem = (kHalves + 2 * kStages) * kOperand + 1024;  // from a 1024-byte boundary on
@@ -389,12 +389,12 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   const int Hkv = a.kv.kv_heads, P = a.kv.page_size;
   // Each role walks the CTA's units by itself; all meet at the start and at the
   // end of a unit.
-  uint32_t tiles_done = 0;         // of the units before: the barriers' phases
-  uint32_t half_done[2] = {0, 0};  // step pairs of each half
+  uint32_t tiles_done = 0;  // of the units before: the barriers' phases
   if (tid < Shape::kSoftmax) {
     set_registers<Shape::kRegsSoftmax, true>();
     // ---- softmax: a row a thread ----
     const int half = H == 2 ? tid >> 7 : 0;
+    uint32_t pairs_done = 0;  // of this half's steps
     UnitLine<UNIT> line(a, prefix, total, ctas);
     for (Unit u; line.next(u);) {
       const int n = u.n, steps = 2 * n, live_halves = u.live_halves;  // even: each buffer's phases stay in step
@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       {
         const uint32_t t_half = tmem + half * 256 + ((uint32_t)((warp & 3) * 32) << 16), t_o = t_half + 128;
         for (int j = 0; j < steps && half < live_halves; ++j) {
-          const uint32_t buf = j & 1, ph = (half_done[half] + (j >> 1)) & 1, age = (tiles_done + (j >> 1)) % Shape::kAges;
+          const uint32_t buf = j & 1, ph = (pairs_done + (j >> 1)) & 1, age = (tiles_done + (j >> 1)) % Shape::kAges;
           if (!(ok = warp_wait(s_done + 8 * (2 * half + buf), ph))) break;
           tc_fence_after();
           const StepScales scales(page_k[age] + 4 * buf, page_lv[age] + 4 * buf, page_inv[age] + 4 * buf, kf);
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
             m2 = nm;
             l *= f;
             if (j > 0) {  // the sums of the steps before, once their products are complete
-              if (!(ok = warp_wait(pv_done + 8 * (2 * half + 1 - buf), (half_done[half] + ((j - 1) >> 1)) & 1))) break;
+              if (!(ok = warp_wait(pv_done + 8 * (2 * half + 1 - buf), (pairs_done + ((j - 1) >> 1)) & 1))) break;
               tc_fence_after();
 #pragma unroll 1
               for (int b = 0; b < D / 16; ++b) {
@@ -489,11 +489,10 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       }
       if (!ok) failed = 1;
       tiles_done += n;
-      half_done[0] += n;
-      if (live_halves == 2) half_done[1] += n;
+      if (half < live_halves) pairs_done += n;
       {
         const bool mine = n > 0 && half < live_halves;
-        if (mine && ok && !warp_wait(pv_done + 8 * (2 * half + 1), (half_done[half] - 1) & 1)) failed = 1;
+        if (mine && ok && !warp_wait(pv_done + 8 * (2 * half + 1), (pairs_done - 1) & 1)) failed = 1;
         tc_fence_after();
         const bool whole = u.whole;
         const float inv = failed ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);
@@ -528,7 +527,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       if (failed) break;  // the phases are not in step any more
     }
   } else if (tid < Shape::kSoftmax + Shape::kConvert) {
-    set_registers<Shape::kRegsConvert, true>();
+    set_registers<Shape::kRegsConvert, false>();
     // ---- conversion of the tiles' codes ----
     UnitLine<UNIT> line(a, prefix, total, ctas);
     for (Unit u; line.next(u);) {
@@ -542,10 +541,10 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       const int turn = (q >> 2) & 1;
       const uint32_t to_a = place(t0, 2 * q + turn), to_b = place(t0, 2 * q + 1 - turn);
       const uint32_t page_bytes = (uint32_t)P * D;  // of a head
-      uint4 kr[PIECES], vr[PIECES];                 // codes of the next tile
+      uint4 reg[PIECES];                            // k's codes of a tile, then v's
       // A tile starts at a page boundary, so a piece's place in its page is the
       // same in every tile.
-      auto load = [&](const uint8_t* pages, uint32_t age, uint4 (&reg)[PIECES]) {
+      auto load = [&](const uint8_t* pages, uint32_t age) {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
           const int tok = t0 + TURN * j;
@@ -553,7 +552,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
           reg[j] = *reinterpret_cast<const uint4*>(block + ((tok & (P - 1)) * D + q * 16));
         }
       };
-      auto store = [&](uint8_t* to, const uint4 (&reg)[PIECES]) {
+      auto store = [&](uint8_t* to) {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
           const uint32_t x[4] = {reg[j].x, reg[j].y, reg[j].z, reg[j].w};
@@ -569,33 +568,27 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         }
       };
       auto pages_of = [&](uint32_t tile) { return warp_wait(page_full + 8 * (tile % Shape::kAges), (tile / Shape::kAges) & 1); };
-      if (n > 0 && (ok = pages_of(tiles_done))) {
-        load(a.kv.k_pages, tiles_done % Shape::kAges, kr);
-        load(a.kv.v_pages, tiles_done % Shape::kAges, vr);
-      }
+      if (n > 0 && (ok = pages_of(tiles_done))) load(a.kv.k_pages, tiles_done % Shape::kAges);
       for (int i = 0; i < n && ok; ++i) {
-        const uint32_t tile = tiles_done + i, st = tile % ST, use = tile / ST;
-        const uint32_t drop = page_drop[tile % Shape::kAges];
+        const uint32_t tile = tiles_done + i, st = tile % ST, use = tile / ST, age = tile % Shape::kAges;
+        const uint32_t drop = page_drop[age];
         if (use > 0 && !(ok = warp_wait(k_empty + 8 * st, (use - 1) & 1))) break;
-        store(sk + st * Shape::kOperand, kr);
+        store(sk + st * Shape::kOperand);
         proxy_fence();
         bar_arrive(k_full + 8 * st);
-        if (i + 1 < n) {
-          if (!(ok = pages_of(tile + 1))) break;
-          load(a.kv.k_pages, (tile + 1) % Shape::kAges, kr);
-        }
+        load(a.kv.v_pages, age);
+        if (i + 1 < n && !(ok = pages_of(tile + 1))) break;
+        if (use > 0 && !(ok = warp_wait(v_empty + 8 * st, (use - 1) & 1))) break;
         if (drop) {
 #pragma unroll
           for (int j = 0; j < PIECES; ++j)
-            if (drop >> ((t0 + TURN * j) >> 4) & 1) vr[j] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+            if (drop >> ((t0 + TURN * j) >> 4) & 1) reg[j] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
         }
-        if (use > 0 && !(ok = warp_wait(v_empty + 8 * st, (use - 1) & 1))) break;
-        store(sv + st * Shape::kOperand, vr);
+        store(sv + st * Shape::kOperand);
         proxy_fence();
         bar_arrive(v_full + 8 * st);
-        if (i + 1 < n) load(a.kv.v_pages, (tile + 1) % Shape::kAges, vr);
+        if (i + 1 < n) load(a.kv.k_pages, (tile + 1) % Shape::kAges);
       }
-
       if (!ok) failed = 1;
       tiles_done += n;
       meet<Shape::kWorking>();
