@@ -415,7 +415,8 @@ int tq_paged_dequantize(const tq_paged_kv* kv, const int32_t* ids, int64_t n, vo
  * were before the rows) or lengths[s] - rows of s (counted = 1).  q is
  * [rows, q_heads, head_dim] (TQ_F16 or TQ_BF16, row stride q_stride elements,
  * 16-byte aligned); query head h attends kv head h / (q_heads / kv_heads).
- * out [rows, q_heads, head_dim] (q's type, contiguous) =
+ * out [rows, q_heads, head_dim] (q's type, contiguous, 32-byte aligned, as
+ * the workspace has to be) =
  * softmax(scale * q . K^T) V; a row that attends nothing is 0 with lse -inf.
  * lse (nullable) [rows, q_heads] fp32 receives the natural-log sum-exp.
  * Positions whose page is missing are not attended.

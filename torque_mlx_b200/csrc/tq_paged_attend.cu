@@ -598,10 +598,10 @@ int tq_paged_attend(const tq_paged_kv* kv, const tq_paged_batch* batch, const vo
   if (batch->rows > 1 && (q_stride < (int64_t)q_heads * kv->head_dim || q_stride % 8)) return TQ_E_SHAPE;
   if (batch->seqs == 0 || batch->rows == 0 || batch->max_new_tokens == 0) return TQ_OK;
   if (!q || !out) return TQ_E_ARG;
-  if ((uintptr_t)q % 16 || (uintptr_t)out % 16) return TQ_E_SHAPE;
+  if ((uintptr_t)q % 16 || (uintptr_t)out % 32) return TQ_E_SHAPE;
   size_t need = 0;
   tq_paged_attend_workspace_size(kv, q_heads, batch->max_new_tokens, &need);
-  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16) return TQ_E_WORKSPACE;
+  if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 32) return TQ_E_WORKSPACE;
   AttendArgs a = {};
   a.kv = *kv;
   a.bt = *batch;

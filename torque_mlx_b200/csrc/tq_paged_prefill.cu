@@ -169,6 +169,36 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// 32 elements to consecutive addresses (32-byte boundaries), whole sectors a
+// store: a thread writes a row of its own, so narrower stores would send every
+// sector twice.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void store_sectors(float* p, const float (&v)[32]) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 8) {
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(v[k + i]);
+    store32(p + k, r);
+  }
+}
+template <typename T> __device__ __forceinline__ void store_sectors(T* p, const float (&v)[32]) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 16) {
+    uint32_t r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T lo = from_f32<T>(v[k + 2 * i]), hi = from_f32<T>(v[k + 2 * i + 1]);
+      r[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+    }
+    store32(p + k, r);
+  }
+}
+
 template <int D> struct PrefillShape {
   static constexpr int kHalves = D == 256 ? 1 : 2;
   static constexpr int kUnit = kHalves * kRows;            // query rows of a unit
@@ -407,34 +437,49 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         const T* row = reinterpret_cast<const T*>(a.q) + (u.first + r / a.group) * a.q_stride +
                        (int64_t)(u.h * a.group + r % a.group) * D;
         uint8_t* sq = smem + half * Shape::kOperand;
-        float up = a.scale2 < 0.f ? -1.f : 1.f, down = 1.f;
-        if (!Exact<T>::fp16) {
-          float top = 0.f;
-          if (live) {
-#pragma unroll 4
-            for (int q = 0; q < D / 8; ++q) {
-              float f[8];
-              load8(row + 8 * q, f);
+        // 64 elements' loads at once, so that their latency is paid once for them
+        constexpr int PARTS = D / 64, VECS = 8;
+        float up = a.scale2 < 0.f ? -1.f : 1.f, down = 1.f, top = 0.f;
+        uint4 x[VECS];
+        auto load_part = [&](int part) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (fabsf(f[k]) <= 3.402823466e38f) top = fmaxf(top, fabsf(f[k]));
-            }
+          for (int q = 0; q < VECS; ++q) {
+            x[q] = make_uint4(0, 0, 0, 0);
+            if (live) x[q] = reinterpret_cast<const uint4*>(row)[part * VECS + q];
+          }
+        };
+        if (!Exact<T>::fp16) {
+#pragma unroll
+          for (int part = PARTS - 1; part >= 0; --part) {
+            load_part(part);
+#pragma unroll
+            for (int q = 0; q < VECS; ++q)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float f = fabsf(to_f32<T>(reinterpret_cast<const T*>(&x[q])[k]));
+                if (f <= 3.402823466e38f) top = fmaxf(top, f);
+              }
           }
           int e = top > 0.f ? 13 - (ilogbf(top) + 1) : 0;
           e = min(120, max(-120, e));
           up *= __int_as_float((e + 127) << 23);
           down = __int_as_float((127 - e) << 23);
         }
-#pragma unroll 4
-        for (int q = 0; q < D / 8; ++q) {
-          float f[8] = {};
-          if (live) load8(row + 8 * q, f);
-          uint4 v;
-          v.x = half2_bits(f[0] * up, f[1] * up);
-          v.y = half2_bits(f[2] * up, f[3] * up);
-          v.z = half2_bits(f[4] * up, f[5] * up);
-          v.w = half2_bits(f[6] * up, f[7] * up);
-          *reinterpret_cast<uint4*>(sq + place(tid & 127, q)) = v;
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) {
+          if (Exact<T>::fp16 || part > 0) load_part(part);
+#pragma unroll
+          for (int q = 0; q < VECS; ++q) {
+            float f[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] = to_f32<T>(reinterpret_cast<const T*>(&x[q])[k]) * up;
+            uint4 v;
+            v.x = half2_bits(f[0], f[1]);
+            v.y = half2_bits(f[2], f[3]);
+            v.z = half2_bits(f[4], f[5]);
+            v.w = half2_bits(f[6], f[7]);
+            *reinterpret_cast<uint4*>(sq + place(tid & 127, part * VECS + q)) = v;
+          }
         }
         kf = fabsf(a.scale2) * down;
         limit = u.base + r / a.group;
@@ -507,13 +552,9 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
           if (mine) tmem_load32(t_o + b * 32, v);
           if (tid < u.nr) {
 #pragma unroll
-            for (int k = 0; k < 32; k += 8) {
-              float f[8];
-#pragma unroll
-              for (int x = 0; x < 8; ++x) f[x] = mine ? v[k + x] * inv : 0.f;
-              if (whole) store8(reinterpret_cast<T*>(a.out) + (row * a.q_heads + hq) * D + b * 32 + k, f);
-              else store8(a.part_o + part * D + b * 32 + k, f);
-            }
+            for (int k = 0; k < 32; ++k) v[k] = mine ? v[k] * inv : 0.f;
+            if (whole) store_sectors(reinterpret_cast<T*>(a.out) + (row * a.q_heads + hq) * D + b * 32, v);
+            else store_sectors(a.part_o + part * D + b * 32, v);
           }
         }
         if (tid < u.nr) {
@@ -725,16 +766,20 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   }
 }
 
-// grid (seqs * kv_heads * tiles, rows / 8): a warp joins the parts of a query row.
+// grid (seqs * kv_heads * tiles, rows / 32): a warp joins the parts of four
+// query rows, whose loads run side by side.
+constexpr int kJoinRows = 4;
+
 template <int D, typename T>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const AttendArgs a, int tiles) {
-  constexpr int UNIT = PrefillShape<D>::kUnit;
+  constexpr int UNIT = PrefillShape<D>::kUnit, R = kJoinRows;
   extern __shared__ __align__(1024) uint8_t prefill_smem[];
   int64_t* prefix = reinterpret_cast<int64_t*>(prefill_smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tile = blockIdx.x % tiles, h = (blockIdx.x / tiles) % a.kv.kv_heads, s = blockIdx.x / tiles / a.kv.kv_heads;
   const SeqWork w = seq_work<UNIT, kTokens>(a, s);
-  const bool any = tile < w.tiles && tile * UNIT + (int)blockIdx.y * 8 < w.n * a.group;
+  const int rows = w.n * a.group - tile * UNIT;  // of this unit, at most UNIT of them
+  const bool any = tile < w.tiles && (int)blockIdx.y * 8 * R < rows;
   int64_t total = 1, ctas = 1, u0 = 0;
   if (any) {
     plan_prefix<UNIT, kTokens, 256>(a, prefix);
@@ -743,51 +788,72 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const AttendArg
     u0 = prefix[s] + ((int64_t)h * w.tiles + tile) * w.weight;
   }
   grid_wait();
-  const int in_tile = blockIdx.y * 8 + warp, r = tile * UNIT + in_tile;
-  if (!any || r >= w.n * a.group) return;
+  const int r0 = (blockIdx.y * 8 + warp) * R;  // first row, in the unit
+  if (!any || r0 >= rows) return;
   const int first = (int)(((u0 + 1) * ctas - 1) / total), last = (int)(((u0 + w.weight) * ctas - 1) / total);
   if (first == last) return;  // finished by its CTA
-  const int n = last - first + 1;
+  const int n = last - first + 1, live = min(R, rows - r0);
   const int slot0 = (int64_t)first * total / ctas < u0 ? 1 : 0;
-  auto part_of = [&](int i) { return ((int64_t)(first + i) * 2 + (i == 0 ? slot0 : 0)) * UNIT + in_tile; };
+  auto part_of = [&](int i, int k) {  // a row past the last one reads that one again
+    return ((int64_t)(first + i) * 2 + (i == 0 ? slot0 : 0)) * UNIT + r0 + min(k, live - 1);
+  };
   constexpr int E = D / 32;  // elements of a lane: pairs at 2 lane, 64 apart
-  float top = -INFINITY, sum = 0.f, v[E];
+  float top[R], sum[R], v[R][E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 32) {  // a lane holds a part's sum; the parts' rows do not wait for it
-    const float mine = i0 + lane < n ? a.part_l[part_of(i0 + lane)] : -INFINITY;
-    float high = mine;
+  for (int k = 0; k < R; ++k) {
+    top[k] = -INFINITY, sum[k] = 0.f;
 #pragma unroll
-    for (int o = 16; o; o >>= 1) high = fmaxf(high, __shfl_xor_sync(FULL, high, o));
-    high = fmaxf(high, top);
-    if (high == -INFINITY) high = 0.f;
-    const float old = ex2(top - high), f = ex2(mine - high);
-    top = high;
-    sum *= old;
+    for (int e = 0; e < E; ++e) v[k][e] = 0.f;
+  }
+  for (int i0 = 0; i0 < n; i0 += 32) {  // a lane holds a part's sum of each row; the rows' elements do not wait for it
+    float f[R];
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] *= old;
-#pragma unroll 4
+    for (int k = 0; k < R; ++k) f[k] = i0 + lane < n ? a.part_l[part_of(i0 + lane, k)] : -INFINITY;
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      float high = f[k];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) high = fmaxf(high, __shfl_xor_sync(FULL, high, o));
+      high = fmaxf(high, top[k]);
+      if (high == -INFINITY) high = 0.f;
+      const float old = ex2(top[k] - high);
+      f[k] = ex2(f[k] - high);
+      top[k] = high;
+      sum[k] *= old;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[k][e] *= old;
+    }
+#pragma unroll 2
     for (int i = i0; i < min(n, i0 + 32); ++i) {
-      const float2* o = reinterpret_cast<const float2*>(a.part_o + part_of(i) * D) + lane;
-      const float fi = __shfl_sync(FULL, f, i - i0);
-      sum += fi;
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 x = o[e * 16];
-        v[e] = fmaf(fi, x.x, v[e]);
-        v[e + 1] = fmaf(fi, x.y, v[e + 1]);
+      for (int k = 0; k < R; ++k) {
+        const float2* o = reinterpret_cast<const float2*>(a.part_o + part_of(i, k) * D) + lane;
+        const float fi = __shfl_sync(FULL, f[k], i - i0);
+        sum[k] += fi;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          const float2 x = o[e * 16];
+          v[k][e] = fmaf(fi, x.x, v[k][e]);
+          v[k][e + 1] = fmaf(fi, x.y, v[k][e + 1]);
+        }
       }
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t row = w.first + r / a.group, hq = h * a.group + r % a.group;
-  T* out = reinterpret_cast<T*>(a.out) + (row * a.q_heads + hq) * D + 2 * lane;
 #pragma unroll
-  for (int e = 0; e < E; e += 2) {
-    out[e * 32] = from_f32<T>(v[e] * inv);
-    out[e * 32 + 1] = from_f32<T>(v[e + 1] * inv);
+  for (int k = 0; k < R; ++k) {
+    if (k >= live) break;
+    const int r = tile * UNIT + r0 + k;
+    const float inv = sum[k] == 0.f ? 0.f : 1.f / sum[k];
+    const int64_t row = w.first + r / a.group, hq = h * a.group + r % a.group;
+    uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + (row * a.q_heads + hq) * D) + lane;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const T lo = from_f32<T>(v[k][e] * inv), hi = from_f32<T>(v[k][e + 1] * inv);
+      out[e * 16] = (uint32_t)*reinterpret_cast<const uint16_t*>(&lo) | (uint32_t)*reinterpret_cast<const uint16_t*>(&hi) << 16;
+    }
+    if (a.lse && lane == 0)
+      a.lse[row * a.q_heads + hq] = sum[k] == 0.f ? -INFINITY : (top[k] + __log2f(sum[k])) * 0.69314718f;
   }
-  if (a.lse && lane == 0) a.lse[row * a.q_heads + hq] = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * 0.69314718f;
 }
 
 size_t prefill_workspace(int head_dim) {
@@ -825,7 +891,7 @@ int launch_prefill_kernel(AttendArgs a, int64_t max_context, cudaStream_t stream
                                   PrefillShape<D>::kSmem + prefix_bytes, stream, a);
   if (st != TQ_OK || a.ctas == 1 || a.whole) return st;
   const int64_t rows = (int64_t)a.bt.max_new_tokens * a.group;
-  const unsigned y = (unsigned)((rows < UNIT ? rows : UNIT) + 7) / 8;
+  const unsigned y = (unsigned)((rows < UNIT ? rows : UNIT) + 8 * kJoinRows - 1) / (8 * kJoinRows);
   return launch_dependent(paged_prefill_join_kernel<D, T>, dim3((unsigned)units, y), dim3(256), prefix_bytes,
                           stream, a, tiles);
 }

@@ -190,12 +190,12 @@ tq_paged_batch batch_of(const Cache& c, int64_t rows, PyObject* lengths_o, PyObj
   return b;
 }
 
-at::Tensor output(PyObject* out_o, at::IntArrayRef shape, at::ScalarType type, int device) {
+at::Tensor output(PyObject* out_o, at::IntArrayRef shape, at::ScalarType type, int device, int align) {
   if (!given(out_o)) return at::empty(shape, at::TensorOptions().dtype(type).device(at::kCUDA, device));
   const at::Tensor& out = tensor(out_o, "out");
   if (out.sizes() != shape || out.scalar_type() != type || !on(out, device) || !out.is_contiguous())
     refuse("out must be contiguous ", type, " ", shape, " on cuda:", device);
-  if (reinterpret_cast<uintptr_t>(out.data_ptr()) % 16) refuse("out must start at a 16-byte boundary");
+  if (reinterpret_cast<uintptr_t>(out.data_ptr()) % align) refuse("out must start at a ", align, "-byte boundary");
   return out;
 }
 
@@ -229,7 +229,7 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     const c10::cuda::OptionalCUDAGuard guard(at::Device(at::kCUDA, c.device));
     qkv = rows_of(qkv);
-    at::Tensor out = output(args[10], {rows, q_heads, d}, qkv.scalar_type(), c.device);
+    at::Tensor out = output(args[10], {rows, q_heads, d}, qkv.scalar_type(), c.device, 16);
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(c.device);
     const bool interleaved = PyObject_IsTrue(args[9]);
     check(unlocked([&] {
@@ -264,7 +264,7 @@ PyObject* paged_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const double scale = given(args[9]) ? real(args[9], "scale") : 1.0 / std::sqrt((double)d);
     const c10::cuda::OptionalCUDAGuard guard(at::Device(at::kCUDA, c.device));
     q = rows_of(q);
-    at::Tensor out = output(args[11], {rows, q_heads, d}, type, c.device), lse;
+    at::Tensor out = output(args[11], {rows, q_heads, d}, type, c.device, 32), lse;
     if (want_lse) lse = at::empty({rows, q_heads}, q.options().dtype(at::kFloat));
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(c.device);
     size_t need = 0;
