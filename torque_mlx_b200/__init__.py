@@ -60,10 +60,11 @@ from .artifact import (  # noqa: E402
     load_torque_artifact,
 )
 from .paged import PagedKV8Cache  # noqa: E402
+from .serving import PagedDecoder  # noqa: E402
 from .verify import verify_drafts  # noqa: E402
 from .w4 import W4Weight, gemv_w4, quantize_w4  # noqa: E402
 from .conversion import FusedAttentionWeights, fuse_attention_weights  # noqa: E402
 
-__all__ += ["FusedAttentionWeights", "PagedKV8Cache", "TorqueArtifact", "TorqueArtifactManifest", "build_torque_artifact",
+__all__ += ["FusedAttentionWeights", "PagedDecoder", "PagedKV8Cache", "TorqueArtifact", "TorqueArtifactManifest", "build_torque_artifact",
             "W4Weight", "convert_npz_checkpoint", "fuse_attention_weights", "gemv_w4", "load_torque_artifact", "quantize_w4",
             "verify_drafts"]
