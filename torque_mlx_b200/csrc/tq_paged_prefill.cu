@@ -207,6 +207,7 @@ template <int D> struct PrefillShape {
   static constexpr int kConvert = D == 256 ? 256 : 128;
   static constexpr int kThreads = 512;                     // four warpgroups, not all warps of the last one working
   static constexpr int kWorking = kSoftmax + kConvert + 32 + kHalves * 32;
+  static constexpr int kMeeting = kSoftmax + kHalves * 32;    // softmax and products: they meet around a unit
   // Registers of a thread, of 128 at launch: softmax, conversion, the rest.
   static constexpr int kRegsSoftmax = 168, kRegsConvert = 96, kRegsRest = 72;
   static_assert(kHalves * kRegsSoftmax + kConvert / 128 * kRegsConvert + kRegsRest <= 4 * 128, "more than the launch's");
@@ -417,8 +418,9 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   const uint32_t tmem = tmem_at;  // half i: S buffers at 256 i and 256 i + 64, O at 256 i + 128
 
   const int Hkv = a.kv.kv_heads, P = a.kv.page_size;
-  // Each role walks the CTA's units by itself; all meet at the start and at the
-  // end of a unit.
+  // Each role walks the CTA's units by itself.  Softmax and products meet at the
+  // start and at the end of a unit (Q and the accumulators change hands); the
+  // others run ahead into the next one as far as the tiles' buffers allow.
   uint32_t tiles_done = 0;  // of the units before: the barriers' phases
   if (tid < Shape::kSoftmax) {
     set_registers<Shape::kRegsSoftmax, true>();
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         free_to = u.base + (u.r0 + half * kRows) / a.group;  // positions up to here need no mask
         proxy_fence();
       }
-      meet<Shape::kWorking>();  // Q is complete
+      meet<Shape::kMeeting>();  // Q is complete
       bool ok = true;
       float m2 = kNoScore, l = 0.f;
       {
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         }
       }
       tc_fence_before();
-      meet<Shape::kWorking>();  // the accumulators have been read
+      meet<Shape::kMeeting>();  // the accumulators have been read
       tc_fence_after();
       if (failed) break;  // the phases are not in step any more
     }
@@ -573,7 +575,6 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
     UnitLine<UNIT> line(a, prefix, total, ctas);
     for (Unit u; line.next(u);) {
       const int n = u.n;
-      meet<Shape::kWorking>();
       bool ok = true;
       constexpr int PIECES = Shape::kPieces, TURN = Shape::kTurn;
       const int pt = tid - Shape::kSoftmax, t0 = pt / Shape::kRow, q = pt % Shape::kRow;
@@ -632,8 +633,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       }
       if (!ok) failed = 1;
       tiles_done += n;
-      meet<Shape::kWorking>();
-      if (failed) break;
+      if (!ok) break;
     }
   } else {
     set_registers<Shape::kRegsRest, false>();
@@ -642,7 +642,6 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       UnitLine<UNIT> line(a, prefix, total, ctas);
       for (Unit u; line.next(u);) {
         const int n = u.n;
-        meet<Shape::kWorking>();
         bool ok = true;
         float most = -INFINITY;  // log2 of the largest v scale so far
         auto find = [&](int i) {
@@ -681,8 +680,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
 
         if (!ok) failed = 1;
         tiles_done += n;
-        meet<Shape::kWorking>();
-        if (failed) break;
+        if (!ok) break;
       }
     } else if (warp >= kIssuer && warp < kIssuer + H) {
       // ---- products of a half: S of two steps, then P V of each step and the S after the next ----
@@ -695,7 +693,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       for (Unit u; line.next(u);) {
         const int n = u.n;
         const bool mine = x < u.live_halves, alone = H == 2 && u.live_halves == 1;
-        meet<Shape::kWorking>();
+        meet<Shape::kMeeting>();
         tc_fence_after();
         bool ok = true;
         // a tile is given back by both halves; the only one at work arrives for both
@@ -751,7 +749,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         if (!ok) failed = 1;
         tiles_done += n;
         if (mine) pairs_done += n;
-        meet<Shape::kWorking>();
+        meet<Shape::kMeeting>();
         tc_fence_after();
         if (failed) break;
       }
