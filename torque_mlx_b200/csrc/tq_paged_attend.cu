@@ -24,6 +24,10 @@
 // CTAs, whatever the sequences' lengths (read on the device, so a captured
 // step follows them).  A unit that falls within one CTA is finished there; the
 // parts of a divided one meet in a second launch.
+//
+// Measured: 64 sequences of 16K to 32K tokens, 32 heads over 8 of 128: 482 to
+// 507 us by the card (6.3 to 6.6 TB/s of codes); one of 131072, 16 heads over 2 of 256: 34 us (4.0 TB/s);
+// one of 512, 8 heads of 128: 7.2 us, of which two launches' latency is most.
 #include "tq_paged_attend.cuh"
 
 namespace tq {
@@ -32,8 +36,12 @@ constexpr int kAttendWarps = 4;
 constexpr int kAttendThreads = kAttendWarps * 32;
 constexpr int kChunk = 16;    // tokens of a ring stage
 constexpr int kMinChunks = 8; // smallest share of a CTA
-constexpr int kWholeChunks = 32;
-
+// What a unit costs besides its chunks (its query rows, the first copies, the
+// warps' parts), in chunks of its CTA.  100 sequences of 1 to 1000 tokens and 8
+// heads take 80 us with 0, 51 with 4, 39 with 8, 33 with 16; 64 of 16K to 32K
+// take 482 to 485 with each of the last three.
+constexpr int kLead = 16;
+constexpr int kWholeFew = 16, kWholeMany = 32;  // chunks up to which units stay whole
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -91,7 +99,7 @@ paged_attend_kernel(const AttendArgs a) {
   const int Hkv = a.kv.kv_heads, P = a.kv.page_size;
 
   grid_wait();
-  plan_prefix<ROWS, kChunk, kAttendThreads>(a, prefix);
+  plan_prefix<ROWS, kChunk, kLead, kAttendThreads>(a, prefix);
   grid_trigger();
   const int64_t total = prefix[a.bt.seqs];
   const int64_t ctas = used_ctas<kMinChunks>(a, total);
@@ -105,15 +113,16 @@ paged_attend_kernel(const AttendArgs a) {
 
   for (int slot = 0; pos < end; slot = 1) {
     const int s = find_seq(prefix, a.bt.seqs, pos);
-    const SeqWork w = seq_work<ROWS, kChunk>(a, s);
+    const SeqWork w = seq_work<ROWS, kChunk, kLead>(a, s);
     const int64_t rel = pos - prefix[s];
-    const int unit = (int)(rel / w.weight), c0 = (int)(rel - (int64_t)unit * w.weight);
-    const int c1 = a.whole ? w.chunks : (int)min((int64_t)w.chunks, c0 + (end - pos));
+    const int unit = (int)(rel / w.weight);
+    int c0, c1;
+    pos += chunk_span(a, w, (int)(rel - (int64_t)unit * w.weight), end - pos, c0, c1);
+    if (c0 == c1) break;  // the share ends in the unit's lead
     const int h = unit / w.tiles, r0 = (unit - h * w.tiles) * ROWS;
     const int nr = min(ROWS, w.n * a.group - r0);             // rows of this tile
     const int last = w.base + (r0 + nr - 1) / a.group;        // last position that any of them attends
     const int free_to = w.base + r0 / a.group;                // positions up to here need no mask
-    pos += a.whole ? 1 : c1 - c0;
 
     // ---- the warp's chunks: c0 + warp, c0 + warp + 4, ... ----
     const int steps = min(c1, last / kChunk + 1) > c0 + warp && last >= 0
@@ -401,8 +410,10 @@ paged_attend_kernel(const AttendArgs a) {
 
 // grid (seqs * kv_heads * tiles, rows, d / DIMS): joins the parts of DIMS
 // elements of one query row.  Few units have many parts each: 256 threads read
-// sixteen of them side by side, 64 elements a CTA.  More units have a few: a
-// CTA of 64 threads for a row.
+// sixteen of them side by side, 64 elements a CTA (one sequence of 131072: 33.7
+// us with the attention, 48.9 with the small CTAs).  More units have a few: a
+// CTA of 64 threads for a row (16 sequences of up to 4001: 13.4 us, 15.5 with
+// the large ones).
 constexpr int kMaxCtas = 148 * 8;
 
 template <int D, int ROWS, int DIMS, int THREADS, typename T>
@@ -418,18 +429,18 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(const AttendArgs a,
   // The attention's CTAs start this kernel after their own wait, so what came
   // before them (the lengths among it) is complete; their parts are read after
   // the wait here, which every CTA makes.
-  const SeqWork w = seq_work<ROWS, kChunk>(a, s);
+  const SeqWork w = seq_work<ROWS, kChunk, kLead>(a, s);
   const bool live = tile < w.tiles && tile * ROWS + r < w.n * a.group;
   int64_t total = 1, ctas = 1, u0 = 0;
   if (live) {
-    plan_prefix<ROWS, kChunk, THREADS>(a, prefix);
+    plan_prefix<ROWS, kChunk, kLead, THREADS>(a, prefix);
     total = prefix[a.bt.seqs];
     ctas = used_ctas<kMinChunks>(a, total);
     u0 = prefix[s] + ((int64_t)h * w.tiles + tile) * w.weight;
   }
   grid_wait();
   if (!live) return;
-  const int first = (int)(((u0 + 1) * ctas - 1) / total), last = (int)(((u0 + w.weight) * ctas - 1) / total);
+  const int first = (int)(((u0 + w.lead + 1) * ctas - 1) / total), last = (int)(((u0 + w.weight) * ctas - 1) / total);
   if (first == last) return;  // finished by its CTA
   const int n = last - first + 1;
   const int slot0 = (int64_t)first * total / ctas < u0 ? 1 : 0;
@@ -529,10 +540,12 @@ int launch_attend(AttendArgs a, int64_t max_context, cudaStream_t stream) {
   const int64_t units = (int64_t)a.bt.seqs * a.kv.kv_heads * tiles;
   if (units > INT32_MAX) return TQ_E_SHAPE;
   const int64_t chunks = (max_context + kChunk - 1) / kChunk;
-  // Units of a few hundred tokens are not divided: the parts' launch would cost
-  // more than the eight steps of a warp that it saves.
-  a.whole = chunks <= kWholeChunks;
-  const int64_t most = a.whole ? units : units * chunks / kMinChunks + 1;
+  // Short units are not divided, since the parts' launch would cost more than
+  // it saves: 8 heads of 251 tokens take 6.2 us whole and 7.2 divided, of 501
+  // 8.6 and 7.2.  Where many units fill the CTAs anyway, longer ones stay whole
+  // too: 512 units of 501 tokens take 17.4 us and 23.4.
+  a.whole = chunks <= (units * 4 >= a.ctas ? kWholeMany : kWholeFew);
+  const int64_t most = a.whole ? units : units * (kLead + chunks) / kMinChunks + 1;
   if (most < a.ctas) a.ctas = (int)most;
   int st = launch_dependent(paged_attend_kernel<D, NT, T>, dim3(a.ctas), dim3(kAttendThreads), smem, stream, a);
   if (st != TQ_OK || a.ctas == 1 || a.whole) return st;
@@ -563,7 +576,10 @@ int launch_dim(const AttendArgs& a, int nt, int64_t max_context, cudaStream_t st
 constexpr int kPrefillFrom = 41;
 inline bool many_rows(int64_t max_new, int group) { return max_new * group >= kPrefillFrom; }
 
-// tiles of 8 query rows, or 16 where a sequence brings more than 8 for a kv head
+// Tiles of 8 query rows, or 16 where a sequence brings more than 8 for a kv
+// head.  8 sequences of 32000 tokens and 8 heads of 128 take 173 us with 12 rows
+// in tiles of 8 and 111 in tiles of 16, with 20 rows 229 and 209; of 1000 tokens
+// 15.0 and 16.8.  4 rows over 16K to 32K tokens take 79 us and 94.
 inline int attend_nt(int64_t max_new, int group) { return max_new * group <= 8 ? 1 : 2; }
 
 }  // namespace tq

@@ -3,9 +3,9 @@
 //
 // The chunks of all units (sequence, kv head, tile of query rows) form one
 // line that is cut evenly over the CTAs, whatever the sequences' lengths (read
-// on the device, so a captured step follows them).  A unit that falls within
-// one CTA is finished there; the parts of a divided one meet in a second
-// launch.
+// on the device, so a captured step follows them).  Each unit's stretch starts
+// with a lead that stands for its fixed cost.  A unit that falls within one CTA
+// is finished there; the parts of a divided one meet in a second launch.
 #pragma once
 
 #include "tq_paged.cuh"
@@ -37,10 +37,11 @@ struct SeqWork {
   int n, base;    // rows; position of the first one
   int tiles;      // query tiles of a kv head
   int chunks;     // chunks of a unit
-  int weight;     // its length on the line: its chunks, or 1 where units are not divided
+  int lead;       // what a unit costs besides its chunks, in chunks
+  int weight;     // its length on the line: lead and chunks, or 1 where units are not divided
 };
 
-template <int ROWS, int CHUNK>
+template <int ROWS, int CHUNK, int LEAD>
 __device__ __forceinline__ SeqWork seq_work(const AttendArgs& a, int s) {
   const RowSpan r = row_span(a.bt, s);
   // a length past the block table is taken as the whole table
@@ -52,12 +53,23 @@ __device__ __forceinline__ SeqWork seq_work(const AttendArgs& a, int s) {
   w.base = a.counted ? held - r.n : held;
   w.tiles = (int)(((int64_t)r.n * a.group + ROWS - 1) / ROWS);
   w.chunks = max(1, (w.base + r.n + CHUNK - 1) / CHUNK);
-  w.weight = a.whole ? 1 : w.chunks;
+  w.lead = a.whole ? 0 : LEAD;
+  w.weight = a.whole ? 1 : LEAD + w.chunks;
   return w;
 }
 
-// prefix[s] = chunks of all units before sequence s, for s in [0, seqs].
-template <int ROWS, int CHUNK, int THREADS>
+// The chunks [c0, c1) of a unit that lie within [rel, rel + room) of its
+// stretch of the line (none where only its lead does); returns the positions
+// that this takes.
+__device__ __forceinline__ int64_t chunk_span(const AttendArgs& a, const SeqWork& w, int rel, int64_t room, int& c0, int& c1) {
+  const int to = (int)min((int64_t)w.weight, rel + room);
+  c0 = a.whole ? 0 : max(0, rel - w.lead);
+  c1 = a.whole ? w.chunks : max(0, to - w.lead);
+  return to - rel;
+}
+
+// prefix[s] = length of all units before sequence s, for s in [0, seqs].
+template <int ROWS, int CHUNK, int LEAD, int THREADS>
 __device__ __forceinline__ void plan_prefix(const AttendArgs& a, int64_t* prefix) {
   __shared__ int64_t sums[THREADS / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -66,7 +78,7 @@ __device__ __forceinline__ void plan_prefix(const AttendArgs& a, int64_t* prefix
     const int s = base + tid;
     int64_t w = 0;
     if (s < a.bt.seqs) {
-      const SeqWork q = seq_work<ROWS, CHUNK>(a, s);
+      const SeqWork q = seq_work<ROWS, CHUNK, LEAD>(a, s);
       w = (int64_t)q.tiles * a.kv.kv_heads * q.weight;
     }
 #pragma unroll
@@ -94,7 +106,7 @@ __device__ __forceinline__ int64_t used_ctas(const AttendArgs& a, int64_t total)
   return most < 1 ? 1 : (most < ctas ? most : ctas);
 }
 
-// last s with prefix[s] <= x (x < prefix[seqs]): the sequence that holds chunk x
+// last s with prefix[s] <= x (x < prefix[seqs]): the sequence that holds position x
 __device__ __forceinline__ int find_seq(const int64_t* prefix, int seqs, int64_t x) {
   int lo = 0, hi = seqs;  // prefix[lo] <= x < prefix[hi]
   while (hi - lo > 1) {

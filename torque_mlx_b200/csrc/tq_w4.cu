@@ -19,6 +19,10 @@
 // that run's fragments, so they need not wait for one another: a tile that
 // lies within a warp's run is finished in registers, and the pieces of a tile
 // that warps share meet in shared memory once, at the end.
+//
+// Measured: 4 tokens, 151936 x 2048, groups of 64: 36 us (166 MB, 4.6 TB/s;
+// 0.69 instructions a clock and scheduler, the logic pipe 52 % busy); 13 tokens,
+// 12288 x 2048, groups of 32: 8.5 us; one token, 4096 x 2048: 3.9 us.
 #include "tq_paged.cuh"
 
 namespace tq {
