@@ -23,7 +23,7 @@
 // softmax ends, whatever the other half does.
 //
 // Measured: 972 tokens behind 4099, 16 heads over 8 of 128: 69 us, 0.53 PFLOP/s.
-// Within a unit a tile of 256 rows by 128 tokens takes 2.3 us (0.99 PFLOP/s over
+// Within a unit a tile of 256 rows by 128 tokens takes 2.3 us (1.08 PFLOP/s over
 // the card); the query rows take 5 us a unit, the output 4, the join 8.
 #include "tq_paged_attend.cuh"
 
