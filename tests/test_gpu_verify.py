@@ -196,3 +196,15 @@ def test_refusals():
             tq.verify_drafts(*ok, draft_counts=bad)
     accepted, out = tq.verify_drafts(*(x[:0] for x in ok))
     assert accepted.shape == (0,) and out.shape == (0, 3)
+
+
+@pytest.mark.parametrize("B", [1, 14, 15, 400])
+def test_most_of_a_cluster_without_columns(B):
+    """Vocabularies of fewer columns than a cluster has CTAs times eight: those without a share have nothing to do
+    before they hand over their keys, with and without drafts, so they are the first to meet the others' memory."""
+    for i, (T, V) in enumerate([(0, 1), (0, 9), (1, 3), (2, 17), (0, 40), (3, 64)]):
+        args = make(1000 * B + i, B, T, V)
+        for _ in range(5):
+            check(*args)
+        if T:
+            check(*args, counts=torch.zeros(B, dtype=torch.int32, device="cuda"))
