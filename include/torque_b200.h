@@ -426,6 +426,15 @@ int tq_paged_attend_workspace_size(const tq_paged_kv* kv, int q_heads, int max_n
 int tq_paged_attend(const tq_paged_kv* kv, const tq_paged_batch* batch, const void* q, int q_dtype, int64_t q_stride,
                     int q_heads, int counted, float scale, int64_t max_context, void* out, float* lse,
                     void* workspace, size_t workspace_bytes, tq_stream_t stream);
+/* The kernel for many query rows (more than 40 for a kv head) waits within a
+ * CTA for its own copies and products.  A wait that is not met after `tries`
+ * (20000 unless set) of 0.1 ms at most gives up: the rows that it leaves undone
+ * are NaN in out and lse, and the CTA is counted.
+ * tq_paged_attend_gave_up waits for the stream and gives the count of the
+ * current device since the library was loaded (0 unless something is wrong);
+ * TQ_E_ARG in a capture. */
+int tq_paged_attend_wait_limit(uint32_t tries);
+int tq_paged_attend_gave_up(uint32_t* ctas, tq_stream_t stream);
 
 /* ---------------------------------------------------------------------------
  * Linear layers with 4-bit weights, for a few tokens.  New in this build (the

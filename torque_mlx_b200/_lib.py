@@ -83,6 +83,8 @@ SIGNATURES: dict[str, tuple] = {
     "tq_paged_attend_workspace_size": (c_int, [c_void_p, c_int, c_int, POINTER(c_size_t)]),
     "tq_paged_attend": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int, c_int, c_float, c_int64, c_void_p,
                                 c_void_p, c_void_p, c_size_t, c_void_p]),
+    "tq_paged_attend_wait_limit": (c_int, [c_uint32]),
+    "tq_paged_attend_gave_up": (c_int, [POINTER(c_uint32), c_void_p]),
     "tq_w4_sizes": (c_int, [c_int64, c_int64, c_int, POINTER(c_size_t), POINTER(c_size_t)]),
     "tq_w4_layout": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
     "tq_w4_quantize": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),

@@ -29,6 +29,7 @@ struct AttendArgs {
   int counted;
   int ctas;
   int whole;       // units are not divided
+  uint32_t tries;  // after which a wait of the kernel for many rows gives up
   float scale2;    // softmax scale times log2(e)
 };
 

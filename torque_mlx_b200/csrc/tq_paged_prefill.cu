@@ -25,6 +25,8 @@
 // Measured: 972 tokens behind 4099, 16 heads over 8 of 128: 69 us, 0.53 PFLOP/s.
 // Within a unit a tile of 256 rows by 128 tokens takes 2.3 us (1.08 PFLOP/s over
 // the card); the query rows take 5 us a unit, the output 4, the join 8.
+#include <atomic>
+
 #include "tq_paged_attend.cuh"
 
 namespace tq {
@@ -45,9 +47,13 @@ __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+constexpr uint32_t kTries = 20000;  // of 0.1 ms at most, before a wait gives up
+std::atomic<uint32_t> wait_tries{kTries};
+__device__ uint32_t gave_up_ctas;   // CTAs that left units undone because a wait gave up
+
 // false if the wait gave up
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
-  for (uint32_t it = 0; it < 20000u; ++it) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, uint32_t tries) {
+  for (uint32_t it = 0; it < tries; ++it) {
     uint32_t done;
     asm volatile(
         "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
@@ -59,7 +65,9 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity) {
   return false;
 }
 // the same for a whole warp, which goes on together
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(FULL, bar_wait(bar, parity)); }
+__device__ __forceinline__ bool all_wait(uint32_t bar, uint32_t parity, uint32_t tries) {
+  return __all_sync(FULL, bar_wait(bar, parity, tries));
+}
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // by the one lane that `lead` picks, of a warp that runs this together
@@ -358,6 +366,16 @@ template <int UNIT> struct UnitLine {
 
 // a barrier of the working warps, wherever they call it
 template <int THREADS> __device__ __forceinline__ void meet() { asm volatile("barrier.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+// the same; true for all of them if it is for any
+template <int THREADS> __device__ __forceinline__ bool meet_any(bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.red.or.pred q, 1, %1, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(any)
+      : "n"(THREADS), "r"((uint32_t)mine)
+      : "memory");
+  return any;
+}
 template <int THREADS> __device__ __forceinline__ void meet_issuers() { asm volatile("barrier.sync 2, %0;" ::"n"(THREADS) : "memory"); }
 template <int REGS, bool MORE> __device__ __forceinline__ void set_registers() {
   if (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
@@ -369,7 +387,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   using Shape = PrefillShape<D>;
   constexpr int H = Shape::kHalves, ST = Shape::kStages, UNIT = Shape::kUnit;
   extern __shared__ __align__(1024) uint8_t prefill_smem[];
-  __shared__ uint64_t bars[4 * ST + 6 * H + 2 * Shape::kAges];
+  __shared__ uint64_t bars[4 * ST + 7 * H + 2 * Shape::kAges];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int failed;
   // of a tile's chunks of sixteen tokens: page and head (0 and a k scale of -1
@@ -386,6 +404,8 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   const uint32_t k_full = bar0, k_empty = k_full + 8 * ST, v_full = k_empty + 8 * ST, v_empty = v_full + 8 * ST;  // [stage]
   const uint32_t s_done = v_empty + 8 * ST, p_full = s_done + 16 * H, pv_done = p_full + 16 * H;  // [half][buffer]
   const uint32_t page_full = pv_done + 16 * H, page_empty = page_full + 8 * Shape::kAges;  // [age]
+  const uint32_t drained = page_empty + 8 * Shape::kAges;                                   // [half]
+  auto warp_wait = [&](uint32_t bar, uint32_t parity) { return all_wait(bar, parity, a.tries); };
 
   grid_wait();
   plan_prefix<UNIT, kTokens, kPrefillLead, Shape::kThreads>(a, prefix);
@@ -409,6 +429,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       bar_init(page_full + 8 * i, 32);
       bar_init(page_empty + 8 * i, H);
     }
+    for (int i = 0; i < H; ++i) bar_init(drained + 8 * i, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     failed = 0;
   }
@@ -429,14 +450,21 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   // Each role walks the CTA's units by itself.  Softmax and products meet at the
   // start and at the end of a unit (Q and the accumulators change hands); the
   // others run ahead into the next one as far as the tiles' buffers allow.
+  //
+  // Every wait has a limit.  A role whose wait gives up sets `failed`; softmax
+  // and products decide together, at the end of a unit, whether any of them saw
+  // that.  If so the rows not reached become NaN (their parts' sums, where the
+  // unit is divided), the products in flight are waited for and the CTA counts
+  // itself; the other roles end at their own waits' limit.
   uint32_t tiles_done = 0;  // of the units before: the barriers' phases
   if (tid < Shape::kSoftmax) {
     set_registers<Shape::kRegsSoftmax, true>();
     // ---- softmax: a row a thread ----
     const int half = H == 2 ? tid >> 7 : 0;
     uint32_t pairs_done = 0;  // of this half's steps
+    bool gave_up = false;
     UnitLine<UNIT> line(a, prefix, total, ctas);
-    for (Unit u; line.next(u);) {
+    for (Unit u; !gave_up && line.next(u);) {
       const int n = u.n, steps = 2 * n, live_halves = u.live_halves;  // even: each buffer's phases stay in step
       float kf = 0.f;  // the row's score factor
       int limit = -1, free_to = 0;
@@ -542,16 +570,16 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
           bar_arrive(p_full + 8 * (2 * half + buf));
         }
       }
-      if (!ok) failed = 1;
       tiles_done += n;
       if (half < live_halves) pairs_done += n;
       {
         const bool mine = n > 0 && half < live_halves;
-        if (mine && ok && !warp_wait(pv_done + 8 * (2 * half + 1), (pairs_done - 1) & 1)) failed = 1;
+        if (mine && ok) ok = warp_wait(pv_done + 8 * (2 * half + 1), (pairs_done - 1) & 1);
+        if (!ok) failed = 1;
         tc_fence_after();
         const bool whole = u.whole;
-        const float inv = failed ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);
-        const float lse = l == 0.f ? -INFINITY : m2 + __log2f(l);
+        const float inv = !ok ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);
+        const float lse = !ok ? __int_as_float(0x7fffffff) : (l == 0.f ? -INFINITY : m2 + __log2f(l));
         const int r = u.r0 + tid;
         const int64_t row = u.first + r / a.group, hq = u.h * a.group + r % a.group;
         const int64_t part = ((int64_t)blockIdx.x * 2 + u.slot) * UNIT + tid;
@@ -573,9 +601,23 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         }
       }
       tc_fence_before();
-      meet<Shape::kMeeting>();  // the accumulators have been read
+      gave_up = meet_any<Shape::kMeeting>(!ok || failed);  // the accumulators have been read
       tc_fence_after();
-      if (failed) break;  // the phases are not in step any more
+    }
+    if (gave_up) {  // the phases are not in step any more: what is left of the share is not computed
+      if (tid == 0) atomicAdd(&gave_up_ctas, 1u);
+      const float nan = __int_as_float(0x7fffffff);
+      for (Unit u; line.next(u);) {
+        if (tid >= u.nr) continue;
+        if (!u.whole) {
+          a.part_l[((int64_t)blockIdx.x * 2 + u.slot) * UNIT + tid] = nan;
+          continue;
+        }
+        const int r = u.r0 + tid;
+        const int64_t at = (u.first + r / a.group) * a.q_heads + u.h * a.group + r % a.group;
+        for (int k = 0; k < D; ++k) reinterpret_cast<T*>(a.out)[at * D + k] = from_f32<T>(nan);
+        if (a.lse) a.lse[at] = nan;
+      }
     }
   } else if (tid < Shape::kSoftmax + Shape::kConvert) {
     set_registers<Shape::kRegsConvert, false>();
@@ -697,8 +739,9 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       const uint64_t q_op = operand(base + x * Shape::kOperand, 16), k_op = operand(k_at, 16), v_op = operand(v_at, 16384);
       const uint32_t s_bar = s_done + 16 * x, p_bar = p_full + 16 * x, pv_bar = pv_done + 16 * x;
       uint32_t pairs_done = 0;  // of this half's steps
+      bool gave_up = false;
       UnitLine<UNIT> line(a, prefix, total, ctas);
-      for (Unit u; line.next(u);) {
+      for (Unit u; !gave_up && line.next(u);) {
         const int n = u.n;
         const bool mine = x < u.live_halves, alone = H == 2 && u.live_halves == 1;
         meet<Shape::kMeeting>();
@@ -757,12 +800,13 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         if (!ok) failed = 1;
         tiles_done += n;
         if (mine) pairs_done += n;
-        meet<Shape::kMeeting>();
+        gave_up = meet_any<Shape::kMeeting>(!ok || failed);
         tc_fence_after();
-        if (failed) break;
       }
-      if (failed)  // products in flight end before the memory goes back
-        for (int i = 0; i < 2; ++i) bar_wait(pv_bar + 8 * i, 0);
+      if (gave_up) {  // products in flight end before the memory goes back
+        tc_commit(drained + 8 * x, lead);
+        all_wait(drained + 8 * x, 0, kTries);
+      }
       meet_issuers<32 * H>();
       if (x == 0) {
         __syncwarp();
@@ -884,6 +928,7 @@ int launch_prefill_kernel(AttendArgs a, int64_t max_context, cudaStream_t stream
   }
   constexpr int UNIT = PrefillShape<D>::kUnit;
   a.ctas = sm_count();
+  a.tries = wait_tries.load(std::memory_order_relaxed);
   a.part_l = a.part_o + (size_t)a.ctas * 2 * UNIT * D;
   const int prefix_bytes = (a.bt.seqs + 1) * (int)sizeof(int64_t);
   const int tiles = (int)(((int64_t)a.bt.max_new_tokens * a.group + UNIT - 1) / UNIT);
@@ -915,3 +960,30 @@ int launch_prefill(const AttendArgs& a, int q_dtype, int64_t max_context, cudaSt
 }
 
 }  // namespace tq
+
+using namespace tq;
+
+extern "C" {
+
+int tq_paged_attend_wait_limit(uint32_t tries) {
+  wait_tries.store(tries, std::memory_order_relaxed);
+  return TQ_OK;
+}
+
+int tq_paged_attend_gave_up(uint32_t* ctas, tq_stream_t stream) {
+  if (!ctas) return TQ_E_ARG;
+  cudaStream_t s = (cudaStream_t)stream;
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  cudaError_t e = cudaStreamIsCapturing(s, &capturing);
+  if (e == cudaSuccess && capturing != cudaStreamCaptureStatusNone) return TQ_E_ARG;
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(ctas, gave_up_ctas, sizeof(*ctas), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    set_last_cuda_error(e);
+    return TQ_E_CUDA;
+  }
+  return TQ_OK;
+}
+
+}  // extern "C"

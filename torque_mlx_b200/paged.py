@@ -20,7 +20,7 @@ tokens that are rejected need no undoing.
 
 from __future__ import annotations
 
-from ctypes import Structure, addressof, c_int32, c_int64, c_void_p
+from ctypes import Structure, addressof, byref, c_int32, c_int64, c_uint32, c_void_p
 
 import torch
 
@@ -123,11 +123,22 @@ class PagedKV8Cache:
         Row t of sequence s sees positions up to ``lengths[s] + t``; with
         ``lengths_counted`` the lengths include the rows.  Returns q's shape and
         type, and with ``return_lse`` also the fp32 natural-log sum-exp
-        ``[rows, q_heads]`` (-inf and a zero row where nothing is seen).
+        ``[rows, q_heads]`` (-inf and a zero row where nothing is seen).  Rows
+        that belong to no sequence leave their part of the results unwritten.
         ``max_context`` (a bound of any sequence's tokens, new ones included)
         sizes the launch; the result does not depend on it."""
         return _lib.binding().paged_attend(self._at, self._index, q, lengths, block_table, token_starts, max_new_tokens,
                                            max_context, lengths_counted, scale, return_lse, out)
+
+    def attend_gave_up(self) -> int:
+        """Thread blocks of many-row attentions on the cache's device that gave
+        up a wait and left NaN behind (tq_paged_attend_gave_up), since the
+        library was loaded: 0 unless something is wrong.  Waits for the current
+        stream."""
+        count = c_uint32()
+        with torch.cuda.device(self.device):
+            _lib.check(_lib.load().tq_paged_attend_gave_up(byref(count), _lib.stream_ptr()), "paged attend")
+        return count.value
 
     # ------------------------------------------------------------ dequantize
     def dequantize(self, page_ids: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16):
