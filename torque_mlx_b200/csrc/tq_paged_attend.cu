@@ -7,7 +7,7 @@
 // score, and v's enters the exponent of a second weight
 // w_j = 2^(s_j + log2(scale_v) - m2), whose reference m2 is kept apart from
 // the softmax's own m, so that pages of very different scale neither overflow
-// nor vanish.  A bf16 query is multiplied by a power of two for each row that
+// nor vanish, and 2^7 lower, so that small weights keep their bits in fp16.  A bf16 query is multiplied by a power of two for each row that
 // takes its largest element to [2^12, 2^13): fp16 then holds it exactly
 // (elements under 2^-30 of the largest are off by 2^-38 of it, less than the
 // roundings of an fp32 product with it).  Only the weights w are rounded,
@@ -276,7 +276,7 @@ paged_attend_kernel(const AttendArgs a) {
           float v = (CHAINS == 1 ? sums[0][nt][k] : sums[0][nt][k] + sums[CHAINS - 1][nt][k]) * (ks * kf[nt][k & 1]);
           if (tok + kChunk - 1 > free_to && tok + g + 8 * (k >> 1) > limit[nt][k & 1]) v = -INFINITY;
           sc[nt][k] = v;
-          grow |= v > m[nt][k & 1] + kLazy || v + lv > m2[nt][k & 1] + kLazy;
+          grow |= v > m[nt][k & 1] + kLazy || v + lv > m2[nt][k & 1] + (kLazy + kRoom);
         }
       if (__any_sync(FULL, grow)) {
 #pragma unroll
@@ -287,7 +287,7 @@ paged_attend_kernel(const AttendArgs a) {
             float top = fmaxf(sc[nt][k], sc[nt][2 + k]);
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
-            const float nm = fmaxf(m[nt][k], top), nm2 = fmaxf(m2[nt][k], top + lv);
+            const float nm = fmaxf(m[nt][k], top), nm2 = fmaxf(m2[nt][k], top + (lv - kRoom));
             l[nt][k] *= ex2(m[nt][k] - nm);
             f2[k] = ex2(m2[nt][k] - nm2);
             m[nt][k] = nm;
@@ -366,13 +366,13 @@ paged_attend_kernel(const AttendArgs a) {
         float top = stat[0][r][0];
 #pragma unroll
         for (int i = 1; i < kAttendWarps; ++i) top = fmaxf(top, stat[i][r][0]);
-        const float f = ex2(m2[nt][k] - top);
+        const float f = ex2(0.5f * (m2[nt][k] - top));  // twice, since the whole factor may be under 2^-126
         float* dst = buf + (warp * ROWS + r) * D;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           // tile mt of a lane: bytes 2mt, 2mt + 1 of its 16 (8 for d = 64) in each 128 (64) of d
           const int dd = D == 64 ? g * 8 + 2 * mt : (mt / 8) * 128 + g * 16 + 2 * (mt % 8);
-          *reinterpret_cast<float2*>(dst + dd) = make_float2(o[mt][nt][k] * f, o[mt][nt][2 + k] * f);
+          *reinterpret_cast<float2*>(dst + dd) = make_float2(o[mt][nt][k] * f * f, o[mt][nt][2 + k] * f * f);
         }
       }
     __syncthreads();

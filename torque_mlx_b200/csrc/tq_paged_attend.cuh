@@ -14,6 +14,11 @@ namespace tq {
 
 constexpr float kNoScore = -1e30f;  // finite, so that differences of two of them are not NaN
 constexpr float kLazy = 8.f;  // a score may pass its reference by 2^8 before the sums are rescaled
+// The weights that fp16 holds are taken against a reference 2^7 under the
+// largest, which with kLazy is all the room that fp16 has above 1 (2^15): it
+// keeps all bits of weights down to 2^-21 of the largest, and 2^-32 of it is
+// what the smaller ones are off by at most.
+constexpr float kRoom = 7.f;
 
 struct AttendArgs {
   tq_paged_kv kv;

@@ -540,8 +540,8 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
           const bool masked = tok + kStep - 1 > free_to;
           const int seen = limit - tok;  // columns 0..seen are visible
           const float top = masked ? highest<true>(v, scales, seen) : highest<false>(v, scales, seen);
-          if (__any_sync(FULL, top > m2 + kLazy)) {
-            const float nm = fmaxf(m2, top), f = ex2(m2 - nm);
+          if (__any_sync(FULL, top > m2 + (kLazy + kRoom))) {
+            const float nm = fmaxf(m2, top - kRoom), f = ex2(m2 - nm);
             m2 = nm;
             l *= f;
             if (j > 0) {  // the sums of the steps before, once their products are complete
