@@ -83,3 +83,58 @@ def test_many_small_weights_beside_large_ones(length, rows, d, drop):
     q = row_of_ones(rows, 1, d, torch.bfloat16)
     out, lse = cache.attend(q, block_table=table, scale=scale, return_lse=True, **batch_args(lens, new))
     check(cache, table, q, lens, new, out, lse, scale)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [6, 60])
+def test_pages_of_much_larger_scale_that_causality_hides(rows, d):
+    """Rows of a first page of ordinary values; what follows, unseen by them, is 2^50 as large."""
+    lens, new = [13], [rows]
+    cache, table = make_cache(72, lens, new, page=16, kv_heads=1, d=d)
+    later = table[0, 1:]
+    cache.value_scales[later[later >= 0].long()] *= 2.0 ** 50
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(rows, 2, d, generator=g, device="cuda").to(torch.bfloat16)
+    out, lse = cache.attend(q, block_table=table, return_lse=True, **batch_args(lens, new))
+    check(cache, table, q, lens, new, out, lse, d ** -0.5)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("rows", [2, 60])
+@pytest.mark.parametrize("small,large,gap", [(-10, 40, 60), (-110, 10, 30), (-100, 100, 150), (-100, 100, 215), (0, 90, 3),
+                                             (-60, 60, 140), (-119, -119, 2), (110, 110, 2)])
+@pytest.mark.parametrize("order", [0, 1])
+def test_scores_that_prefer_the_smaller_values(order, small, large, gap, rows, d):
+    """Pages of value scales 2^small and 2^large by turns, those of the small ones with scores `gap` powers of two above."""
+    lens, new = [300], [rows]
+    cache, table = aimed(73, lens, new, page=16, kv_heads=1, d=d)
+    ids = table[0, :-(-(lens[0] + rows) // 16)].long()
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for i, id_ in enumerate(ids.tolist()):
+        low = (i // 3) % 2 == order
+        cache.value_scales[id_] = 2.0 ** (small if low else large)
+        cache.key_pages[id_, :, :, 0] = (128 + torch.randint(-2, 3, (1, 16), generator=g, device="cuda")
+                                         + (100 if low else 0)).to(torch.uint8)
+    scale = gap * math.log(2) / (100 * 0.01)
+    q = row_of_ones(rows, 1, d, torch.bfloat16)
+    args = dict(block_table=table, scale=scale, **batch_args(lens, new))
+    out, lse = cache.attend(q, return_lse=True, **args)
+    check(cache, table, q, lens, new, out, lse, scale)
+    out = cache.attend(q, max_context=1 << 20, **args)
+    check(cache, table, q, lens, new, out, None, scale)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_small_weights_of_values_without_scale(d):
+    """Pages of zeros (scale 0 or the smallest) hold nearly all the weight: the sum counts them."""
+    lens, new = [150], [60]
+    cache, table = aimed(74, lens, new, page=16, kv_heads=1, d=d)
+    for i, id_ in enumerate(table[0, :14].tolist()):
+        if i % 3 < 2:
+            cache.key_pages[id_, :, :, 0] = 228
+            cache.value_pages[id_] = 128
+            cache.value_scales[id_] = (0.0, 2.0 ** -120)[i % 3]
+    scale = 9 * math.log(2)
+    q = row_of_ones(60, 1, d, torch.float16)
+    out, lse = cache.attend(q, block_table=table, scale=scale, return_lse=True, **batch_args(lens, new))
+    check(cache, table, q, lens, new, out, lse, scale)

@@ -3,9 +3,11 @@
 //
 // Mathematics: as in tq_paged_attend.cu, with one exponential for each score.
 // For a page of 2^lv scale, w_j = 2^(s_j + lv - m2) weighs v's codes, and the
-// softmax's own sum is l = sum_j w_j 2^-lv.  Where a page's scale is under
-// 2^-40 of the largest seen (or 2^-90), its values are left out of the product
-// and lv is taken that large, so that l stays exact.
+// softmax's own sum l = sum_j 2^(s_j - m), whose reference m is kept apart as
+// there, takes a chunk of one page as (sum_j w_j) 2^(m2 - m - lv).  Where that
+// factor is past 2^64 (the row has seen values so much larger that a chunk's w
+// may vanish before its share of l does) or the page's values have no scale at
+// all, the chunk's own exponentials are taken instead.
 //
 // Bound: the two products, 4 d flops for each visible (row, token) pair, on
 // the tensor cores, and the exponentials, which take as long at d = 128 (16 a
@@ -240,46 +242,70 @@ template <int D> struct PrefillShape {
 // byte offset of elements [8 q, 8 q + 8) of row t within an operand
 __device__ __forceinline__ uint32_t place(int t, int q) { return (uint32_t)((q >> 3) * 16384 + t * 128 + (((q & 7) ^ (t & 7)) << 4)); }
 
-// A step's chunks of sixteen tokens as the softmax uses them: scores times f
-// plus the logarithm of v's scale are the exponents, weights times inv count
-// in the softmax's own sum.  Without a page f is 0 and the exponent -inf.
+// A step's chunks of sixteen tokens as the softmax uses them: products times f
+// are the scores, and with the logarithm of v's scale the weights' exponents.
+// Without a page f is negative and the logarithm -inf.
 struct StepScales {
-  float f[4], lv[4], inv[4];
+  float f[4], lv[4];
 
-  __device__ __forceinline__ StepScales(const float* ks, const float* lvs, const float* invs, float kf) {
-    const float4 k = *reinterpret_cast<const float4*>(ks), v = *reinterpret_cast<const float4*>(lvs),
-                 i = *reinterpret_cast<const float4*>(invs);
+  __device__ __forceinline__ StepScales(const float* ks, const float* lvs, float kf) {
+    const float4 k = *reinterpret_cast<const float4*>(ks), v = *reinterpret_cast<const float4*>(lvs);
     f[0] = k.x, f[1] = k.y, f[2] = k.z, f[3] = k.w;
     lv[0] = v.x, lv[1] = v.y, lv[2] = v.z, lv[3] = v.w;
-    inv[0] = i.x, inv[1] = i.y, inv[2] = i.z, inv[3] = i.w;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const bool none = f[c] < 0.f;
-      f[c] = none ? 0.f : f[c] * kf;
-      lv[c] = none ? -INFINITY : lv[c];
-    }
+    for (int c = 0; c < 4; ++c)
+      if (f[c] >= 0.f) f[c] *= kf;
   }
 };
 
-// The largest exponent of a row's step; columns past `seen` are hidden where
-// MASKED.
+// The largest exponent of a row's step, and its largest score; columns past
+// `seen` are hidden where MASKED.
 template <bool MASKED>
-__device__ __forceinline__ float highest(const float (&v)[kStep], const StepScales& w, int seen) {
+__device__ __forceinline__ float highest(const float (&v)[kStep], const StepScales& w, int seen, float& score) {
   float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int k = 0; k < 16; ++k)
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       if (!MASKED || c * 16 + k <= seen) x[c] = fmaxf(x[c], v[c * 16 + k]);
+  // a NaN (nothing visible, or no page) is passed over
+  float s[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) x[c] = fmaf(x[c], w.f[c], w.lv[c]);
-  return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));  // a NaN (nothing visible, or no page) is passed over
+  for (int c = 0; c < 4; ++c) {
+    s[c] = w.f[c] < 0.f ? -INFINITY : x[c] * w.f[c];
+    x[c] = fmaf(x[c], w.f[c], w.lv[c]);
+  }
+  score = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+  return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
 }
 
-// The row's weights to tensor memory, and their sum without v's scales to l.
+// sum_j 2^(s_j - m) of chunk c
 template <bool MASKED>
-__device__ __forceinline__ void weigh(uint32_t at, const float (&v)[kStep], const StepScales& w, float m2, int seen,
+__device__ __forceinline__ float chunk_sum(const float (&v)[kStep], const StepScales& w, int c, float m, int seen) {
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    if (!MASKED || c * 16 + k <= seen) sum += ex2(fmaf(v[c * 16 + k], w.f[c], -m));
+  return sum;
+}
+
+// The row's weights to tensor memory, and the sum of 2^(s - m) to l.
+template <bool MASKED>
+__device__ __forceinline__ void weigh(uint32_t at, const float (&v)[kStep], const StepScales& w, float m, float m2, int seen,
                                       float& l) {
+  float factor[4];
+  bool apart = false;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const float e = m2 - m - w.lv[c];
+    factor[c] = w.f[c] < 0.f || e > 64.f ? 0.f : ex2(e);
+    apart |= w.f[c] >= 0.f && e > 64.f;
+  }
+  if (__any_sync(FULL, apart)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (w.f[c] >= 0.f && m2 - m - w.lv[c] > 64.f) l += chunk_sum<MASKED>(v, w, c, m, seen);
+  }
   float sums[4];
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
@@ -318,7 +344,7 @@ __device__ __forceinline__ void weigh(uint32_t at, const float (&v)[kStep], cons
       sums[2 * b + u] = e.x + e.y;
     }
   }
-  l += fmaf(sums[0], w.inv[0], sums[1] * w.inv[1]) + fmaf(sums[2], w.inv[2], sums[3] * w.inv[3]);
+  l += fmaf(sums[0], factor[0], sums[1] * factor[1]) + fmaf(sums[2], factor[2], sums[3] * factor[3]);
 }
 
 // A part of a unit that falls to a CTA.
@@ -390,10 +416,10 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   __shared__ uint64_t bars[4 * ST + 7 * H + 2 * Shape::kAges];
   __shared__ uint32_t tmem_at;
   __shared__ volatile int failed;
-  // of a tile's chunks of sixteen tokens: page and head (0 and a k scale of -1
-  // where there is no page), scales, and whether v is left out of the product
-  __shared__ uint32_t page_at[Shape::kAges][8], page_drop[Shape::kAges];
-  __shared__ __align__(16) float page_k[Shape::kAges][8], page_lv[Shape::kAges][8], page_inv[Shape::kAges][8];
+  // of a tile's chunks of sixteen tokens: page and head (page 0 and a k scale of
+  // -1 where there is none), k's scale and the logarithm of v's
+  __shared__ uint32_t page_at[Shape::kAges][8];
+  __shared__ __align__(16) float page_k[Shape::kAges][8], page_lv[Shape::kAges][8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t raw = (uint32_t)__cvta_generic_to_shared(prefill_smem), base = (raw + 1023u) & ~1023u;
   uint8_t* const smem = prefill_smem + (base - raw);
@@ -526,25 +552,27 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       }
       meet<Shape::kMeeting>();  // Q is complete
       bool ok = true;
-      float m2 = kNoScore, l = 0.f;
+      float m = kNoScore, m2 = kNoScore, l = 0.f;
       {
         const uint32_t t_half = tmem + half * 256 + ((uint32_t)((warp & 3) * 32) << 16), t_o = t_half + 128;
         for (int j = 0; j < steps && half < live_halves; ++j) {
           const uint32_t buf = j & 1, ph = (pairs_done + (j >> 1)) & 1, age = (tiles_done + (j >> 1)) % Shape::kAges;
           if (!(ok = warp_wait(s_done + 8 * (2 * half + buf), ph))) break;
           tc_fence_after();
-          const StepScales scales(page_k[age] + 4 * buf, page_lv[age] + 4 * buf, page_inv[age] + 4 * buf, kf);
+          const StepScales scales(page_k[age] + 4 * buf, page_lv[age] + 4 * buf, kf);
           float v[kStep];
           tmem_load64(t_half + buf * kStep, v);
           const int tok = u.c0 * kTokens + j * kStep;
           const bool masked = tok + kStep - 1 > free_to;
           const int seen = limit - tok;  // columns 0..seen are visible
-          const float top = masked ? highest<true>(v, scales, seen) : highest<false>(v, scales, seen);
-          if (__any_sync(FULL, top > m2 + (kLazy + kRoom))) {
-            const float nm = fmaxf(m2, top - kRoom), f = ex2(m2 - nm);
-            m2 = nm;
-            l *= f;
-            if (j > 0) {  // the sums of the steps before, once their products are complete
+          float score;
+          const float top = masked ? highest<true>(v, scales, seen, score) : highest<false>(v, scales, seen, score);
+          if (__any_sync(FULL, top > m2 + (kLazy + kRoom) || score > m + kLazy)) {
+            const float nm = fmaxf(m, score), nm2 = fmaxf(m2, top - kRoom), f = ex2(m2 - nm2);
+            l *= ex2(m - nm);
+            m = nm;
+            m2 = nm2;
+            if (j > 0 && __any_sync(FULL, f != 1.f)) {  // the sums of the steps before, once their products are complete
               if (!(ok = warp_wait(pv_done + 8 * (2 * half + 1 - buf), (pairs_done + ((j - 1) >> 1)) & 1))) break;
               tc_fence_after();
 #pragma unroll 1
@@ -563,8 +591,8 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
               }
             }
           }
-          if (masked) weigh<true>(t_half + buf * kStep, v, scales, m2, seen, l);
-          else weigh<false>(t_half + buf * kStep, v, scales, m2, seen, l);
+          if (masked) weigh<true>(t_half + buf * kStep, v, scales, m, m2, seen, l);
+          else weigh<false>(t_half + buf * kStep, v, scales, m, m2, seen, l);
           tmem_store_wait();
           tc_fence_before();
           bar_arrive(p_full + 8 * (2 * half + buf));
@@ -578,8 +606,9 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         if (!ok) failed = 1;
         tc_fence_after();
         const bool whole = u.whole;
-        const float inv = !ok ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : 1.f / l);
-        const float lse = !ok ? __int_as_float(0x7fffffff) : (l == 0.f ? -INFINITY : m2 + __log2f(l));
+        // 2^(m2 - m) / l; its power in two halves, since the whole may be under 2^-126
+        const float up = ex2(0.5f * (m2 - m)), inv = !ok ? __int_as_float(0x7fffffff) : (l == 0.f ? 0.f : up / l);
+        const float lse = !ok ? __int_as_float(0x7fffffff) : (l == 0.f ? -INFINITY : m + __log2f(l));
         const int r = u.r0 + tid;
         const int64_t row = u.first + r / a.group, hq = u.h * a.group + r % a.group;
         const int64_t part = ((int64_t)blockIdx.x * 2 + u.slot) * UNIT + tid;
@@ -590,7 +619,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
           if (mine) tmem_load32(t_o + b * 32, v);
           if (tid < u.nr) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] = mine ? v[k] * inv : 0.f;
+            for (int k = 0; k < 32; ++k) v[k] = mine ? v[k] * inv * up : 0.f;
             if (whole) store_sectors(reinterpret_cast<T*>(a.out) + (row * a.q_heads + hq) * D + b * 32, v);
             else store_sectors(a.part_o + part * D + b * 32, v);
           }
@@ -663,7 +692,6 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       if (n > 0 && (ok = pages_of(tiles_done))) load(a.kv.k_pages, tiles_done % Shape::kAges);
       for (int i = 0; i < n && ok; ++i) {
         const uint32_t tile = tiles_done + i, st = tile % ST, use = tile / ST, age = tile % Shape::kAges;
-        const uint32_t drop = page_drop[age];
         if (use > 0 && !(ok = warp_wait(k_empty + 8 * st, (use - 1) & 1))) break;
         store(sk + st * Shape::kOperand);
         proxy_fence();
@@ -671,11 +699,6 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
         load(a.kv.v_pages, age);
         if (i + 1 < n && !(ok = pages_of(tile + 1))) break;
         if (use > 0 && !(ok = warp_wait(v_empty + 8 * st, (use - 1) & 1))) break;
-        if (drop) {
-#pragma unroll
-          for (int j = 0; j < PIECES; ++j)
-            if (drop >> ((t0 + TURN * j) >> 4) & 1) reg[j] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-        }
         store(sv + st * Shape::kOperand);
         proxy_fence();
         bar_arrive(v_full + 8 * st);
@@ -693,7 +716,6 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
       for (Unit u; line.next(u);) {
         const int n = u.n;
         bool ok = true;
-        float most = -INFINITY;  // log2 of the largest v scale so far
         auto find = [&](int i) {
           const int tok = (u.c0 + i) * kTokens + lane * 16;
           return lane < 8 && i < n && tok <= u.last ? page_id(a.kv, a.bt, u.s, tok / P) : -1;
@@ -709,20 +731,11 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
             ks = a.kv.k_scales[block];
             lv = log2f(a.kv.v_scales[block]);
           }
-          float top = lv;
-#pragma unroll
-          for (int o = 4; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
-          most = fmaxf(most, __shfl_sync(FULL, top, 0));
-          const float least = fmaxf(most - 40.f, -90.f);
-          const uint32_t drop = __ballot_sync(FULL, id >= 0 && lv < least);
           if (use > 0 && !(ok = warp_wait(page_empty + 8 * age, (use - 1) & 1))) break;
           if (lane < 8) {
-            const float use_lv = id < 0 ? 0.f : (lv < least ? least : lv);
             page_at[age][lane] = (uint32_t)block;
             page_k[age][lane] = ks;
-            page_lv[age][lane] = use_lv;
-            page_inv[age][lane] = ex2(-use_lv);
-            if (lane == 0) page_drop[age] = drop;
+            page_lv[age][lane] = lv;
           }
           __syncwarp();
           bar_arrive(page_full + 8 * age);
