@@ -878,9 +878,9 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const AttendArg
 #pragma unroll
       for (int o = 16; o; o >>= 1) high = fmaxf(high, __shfl_xor_sync(FULL, high, o));
       high = fmaxf(high, top[k]);
-      if (high == -INFINITY) high = 0.f;
-      const float old = ex2(top[k] - high);
-      f[k] = ex2(f[k] - high);
+      const float ref = high == -INFINITY ? 0.f : high;  // nothing yet: the next parts may lie far below 0
+      const float old = ex2(top[k] - ref);
+      f[k] = ex2(f[k] - ref);
       top[k] = high;
       sum[k] *= old;
 #pragma unroll
