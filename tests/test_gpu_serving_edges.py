@@ -1,0 +1,46 @@
+"""Serving operators at the edges of what their arguments may be."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import torque_mlx_b200 as tq  # noqa: E402
+
+from test_gpu_paged import make_cache, tables  # noqa: E402
+
+
+def test_rows_repeated_by_a_stride_of_zero():
+    cache, table = make_cache(81, [40, 7, 90], [1, 1, 1], page=16, kv_heads=2, d=64)
+    args = dict(lengths=torch.tensor([40, 7, 90], dtype=torch.int32, device="cuda"), block_table=table)
+    one = torch.randn(1, 8 * 64, device="cuda").to(torch.bfloat16)
+    cos, sin = tables(100, 64)
+    many = one.expand(3, -1)
+    assert torch.equal(cache.append(many, cos, sin, **args), cache.append(many.contiguous(), cos, sin, **args))
+    q = one[:, :256].reshape(1, 4, 64).expand(3, -1, -1)
+    assert torch.equal(cache.attend(q, **args), cache.attend(q.contiguous(), **args))
+    step = torch.randn(8 * 64 + 2 * 8, device="cuda").to(torch.bfloat16).as_strided((3, 8 * 64), (8, 1))  # rows that overlap
+    assert torch.equal(cache.append(step, cos, sin, **args), cache.append(step.contiguous(), cos, sin, **args))
+
+
+@pytest.mark.parametrize("mode", ["plain", "f32", "rms", "silu"])
+def test_product_of_rows_repeated_by_a_stride_of_zero(mode):
+    w = tq.W4Weight.quantize(torch.randn(96, 256, device="cuda"), group_size=64)
+    x = torch.randn(1, 512 if mode == "silu" else 256, device="cuda")
+    x = (x if mode == "f32" else x.to(torch.bfloat16)).expand(5, -1)
+    norm = torch.ones(256, device="cuda", dtype=torch.bfloat16) if mode == "rms" else None
+    assert torch.equal(tq.gemv_w4(w, x, mode=mode, norm_weight=norm), tq.gemv_w4(w, x.contiguous(), mode=mode, norm_weight=norm))
+
+
+def test_verification_of_rows_repeated_by_a_stride_of_zero():
+    g = torch.Generator(device="cuda").manual_seed(4)
+    p = torch.softmax(torch.randn(1, 1, 100, generator=g, device="cuda"), -1)
+    noise = torch.empty(1, 100, device="cuda").exponential_(generator=g)
+    tokens = torch.randint(0, 100, (3, 2), generator=g, device="cuda").to(torch.int32)
+    uniform = torch.rand(3, 2, generator=g, device="cuda")
+    got = tq.verify_drafts(p.expand(3, 3, 100), p.expand(3, 2, 100), tokens, uniform, noise.expand(3, 100))
+    want = tq.verify_drafts(p.expand(3, 3, 100).contiguous(), p.expand(3, 2, 100).contiguous(), tokens, uniform,
+                            noise.expand(3, 100).contiguous())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -84,6 +84,14 @@ int dtype_code(at::ScalarType t) {
 
 bool on(const at::Tensor& t, int device) { return t.is_cuda() && t.get_device() == device; }
 
+// Whether the slices of `t` along `dim` follow one another without overlap (an
+// expanded tensor repeats one).
+bool apart(const at::Tensor& t, int64_t dim) {
+  int64_t inner = 1;
+  for (int64_t d = dim + 1; d < t.dim(); ++d) inner *= t.size(d);
+  return t.size(dim) <= 1 || t.stride(dim) >= inner;
+}
+
 // `t` with contiguous rows (the first dimension's stride free) at 16-byte
 // boundaries, copied only where it has none.
 at::Tensor rows_of(const at::Tensor& t) {
@@ -96,7 +104,7 @@ at::Tensor rows_of(const at::Tensor& t) {
   }
   const bool aligned = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
                        (t.size(0) <= 1 || t.stride(0) * t.element_size() % 16 == 0);
-  return aligned ? t : t.clone(at::MemoryFormat::Contiguous);
+  return aligned && apart(t, 0) ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 // Workspace of one call, from torch's allocator for the current stream and
@@ -321,7 +329,7 @@ PyObject* gemv_w4(PyObject*, PyObject* const* args, Py_ssize_t count) {
     }
     const int64_t tokens = x.dim() == 2 ? x.size(0) : 1;
     const c10::cuda::OptionalCUDAGuard guard(at::Device(at::kCUDA, device));
-    if (width > 1 && x.stride(-1) != 1) x = x.contiguous();
+    if ((width > 1 && x.stride(-1) != 1) || (x.dim() == 2 && !apart(x, 0))) x = x.contiguous();
     const void *norm = nullptr, *residual = nullptr;
     if (mode == 2) {
       if (!given(args[7])) refuse("gemv_w4: mode 'rms' needs norm_weight");
@@ -373,13 +381,13 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const at::ScalarType type = target.scalar_type();
     const int code = dtype_code(type);
     const c10::cuda::OptionalCUDAGuard guard(at::Device(at::kCUDA, device));
-    if (vocab > 1 && target.stride(2) != 1) target = target.contiguous();
+    if ((vocab > 1 && target.stride(2) != 1) || !apart(target, 1)) target = target.contiguous();
     at::Tensor draft;
     if (given(args[1])) {
       draft = tensor(args[1], "draft_probs");
       if (draft.sizes() != at::IntArrayRef({seqs, drafts, vocab}) || draft.scalar_type() != type || !on(draft, device))
         refuse("draft_probs must be ", type, " [", seqs, ", ", drafts, ", ", vocab, "] on cuda:", device);
-      if (vocab > 1 && draft.stride(2) != 1) draft = draft.contiguous();
+      if ((vocab > 1 && draft.stride(2) != 1) || !apart(draft, 1)) draft = draft.contiguous();
     }
     at::Tensor tokens = tensor(args[2], "draft_tokens"), uniform = tensor(args[3], "uniform"),
                noise = tensor(args[4], "noise");
@@ -391,7 +399,7 @@ PyObject* verify_drafts(PyObject*, PyObject* const* args, Py_ssize_t n) {
       refuse("noise must be fp32 [", seqs, ", ", vocab, "] on cuda:", device);
     tokens = tokens.contiguous();
     uniform = uniform.contiguous();
-    if (vocab > 1 && noise.stride(1) != 1) noise = noise.contiguous();
+    if ((vocab > 1 && noise.stride(1) != 1) || !apart(noise, 0)) noise = noise.contiguous();
     const int32_t* counts = nullptr;
     if (given(args[5])) {
       const at::Tensor& t = tensor(args[5], "draft_counts");
