@@ -44,3 +44,11 @@ def test_verification_of_rows_repeated_by_a_stride_of_zero():
     want = tq.verify_drafts(p.expand(3, 3, 100).contiguous(), p.expand(3, 2, 100).contiguous(), tokens, uniform,
                             noise.expand(3, 100).contiguous())
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_out_of_memory_has_its_own_type():
+    """As torch's own allocations have it, so that a server may catch it and shed load."""
+    cache = tq.PagedKV8Cache(1, kv_heads=64, head_dim=256, page_size=128)
+    pages = torch.zeros(1 << 20, dtype=torch.int32, device="cuda")  # 4 TB of values
+    with pytest.raises(torch.OutOfMemoryError):
+        cache.dequantize(pages, dtype=torch.float16)

@@ -128,12 +128,24 @@ PyObject* wrap_pair(at::Tensor a, at::Tensor b) {
   return both;
 }
 
+// torch.OutOfMemoryError, as torch's own calls raise it
+void out_of_memory(const char* what) {
+  PyObject* torch = PyImport_ImportModule("torch");
+  PyObject* type = torch ? PyObject_GetAttrString(torch, "OutOfMemoryError") : nullptr;
+  if (!type) PyErr_Clear();
+  PyErr_SetString(type ? type : PyExc_RuntimeError, what);
+  Py_XDECREF(type);
+  Py_XDECREF(torch);
+}
+
 // Runs `f`, with C++ errors as Python exceptions.
 template <typename F> PyObject* guarded(F f) {
   try {
     return f();
   } catch (const BadArgument& e) {
     PyErr_SetString(PyExc_ValueError, e.what());
+  } catch (const c10::OutOfMemoryError& e) {
+    out_of_memory(e.what_without_backtrace());
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }
