@@ -52,3 +52,15 @@ def test_out_of_memory_has_its_own_type():
     pages = torch.zeros(1 << 20, dtype=torch.int32, device="cuda")  # 4 TB of values
     with pytest.raises(torch.OutOfMemoryError):
         cache.dequantize(pages, dtype=torch.float16)
+
+
+def test_truth_values_that_have_none():
+    cache, table = make_cache(82, [4], [1], page=16, kv_heads=1, d=64)
+    args = dict(lengths=torch.tensor([4], dtype=torch.int32, device="cuda"), block_table=table)
+    both = torch.tensor([True, False])  # has no truth value
+    q = torch.zeros(1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    for kw in (dict(lengths_counted=both), dict(return_lse=both)):
+        with pytest.raises(ValueError):
+            cache.attend(q, **kw, **args)
+    with pytest.raises(ValueError):
+        cache.append(torch.zeros(1, 3 * 64, device="cuda"), interleaved=both, **args)

@@ -74,6 +74,14 @@ double real(PyObject* o, const char* name) {
   }
   return v;
 }
+bool truth(PyObject* o, const char* name) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) {
+    PyErr_Clear();
+    refuse(name, " must be true or false");
+  }
+  return v;
+}
 
 int dtype_code(at::ScalarType t) {
   if (t == at::kFloat) return TQ_F32;
@@ -246,7 +254,7 @@ PyObject* paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     qkv = rows_of(qkv);
     at::Tensor out = output(args[10], {rows, q_heads, d}, qkv.scalar_type(), c.device, 16);
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(c.device);
-    const bool interleaved = PyObject_IsTrue(args[9]);
+    const bool interleaved = truth(args[9], "interleaved");
     check(unlocked([&] {
             return tq_paged_append(c.kv, &b, qkv.data_ptr(), code, qkv.stride(0), (int)q_heads, cos, sin, positions,
                                    (int)rotary, interleaved, out.data_ptr(), stream);
@@ -275,7 +283,7 @@ PyObject* paged_attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
       most_context = integer(args[7], "max_context");
       if (most_context < 0) refuse("max_context must not be negative");
     }
-    const bool counted = PyObject_IsTrue(args[8]), want_lse = PyObject_IsTrue(args[10]);
+    const bool counted = truth(args[8], "lengths_counted"), want_lse = truth(args[10], "return_lse");
     const double scale = given(args[9]) ? real(args[9], "scale") : 1.0 / std::sqrt((double)d);
     const c10::cuda::OptionalCUDAGuard guard(at::Device(at::kCUDA, c.device));
     q = rows_of(q);
