@@ -2,14 +2,17 @@
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 
 import torque_mlx_b200 as tq  # noqa: E402
+from torque_mlx_b200 import _lib  # noqa: E402
 
-from test_gpu_paged import make_cache, tables  # noqa: E402
+from test_gpu_paged import batch_args, make_cache, tables  # noqa: E402
 
 
 def test_rows_repeated_by_a_stride_of_zero():
@@ -64,3 +67,29 @@ def test_truth_values_that_have_none():
             cache.attend(q, **kw, **args)
     with pytest.raises(ValueError):
         cache.append(torch.zeros(1, 3 * 64, device="cuda"), interleaved=both, **args)
+
+
+def test_row_counts_announced_beyond_the_rows():
+    """The largest number that the C ABI takes for `max_new_tokens`: no more rows are there than there are."""
+    from test_paged_abi_cpu import _Batch
+    lens, new = [20, 70], [3, 1]
+    lib = _lib.load()
+    x = torch.randn(4, 8 * 64, device="cuda").to(torch.bfloat16)
+    results = []
+    for most in (3, 2 ** 31 - 1):
+        cache, table = make_cache(83, lens, new, page=16, kv_heads=2, d=64)
+        a = batch_args(lens, new)
+        b = _Batch(table.data_ptr(), a["lengths"].data_ptr(), a["token_starts"].data_ptr(), table.stride(0), 4,
+                   table.shape[1], 2, most)
+        q = torch.empty(4, 4, 64, device="cuda", dtype=torch.bfloat16)
+        out = torch.empty_like(q)
+        need = ctypes.c_size_t()
+        stream = torch.cuda.current_stream().cuda_stream
+        assert lib.tq_paged_append(cache._at, ctypes.byref(b), x.data_ptr(), _lib.TQ_BF16, x.stride(0), 4, None, None, 0, 0, 1,
+                                   q.data_ptr(), stream) == 0
+        assert lib.tq_paged_attend_workspace_size(cache._at, 4, most, ctypes.byref(need)) == 0
+        ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+        assert lib.tq_paged_attend(cache._at, ctypes.byref(b), q.data_ptr(), _lib.TQ_BF16, q.stride(0), 4, 0, 0.125, 128,
+                                   out.data_ptr(), None, ws.data_ptr(), need.value, stream) == 0
+        results.append((q, out, cache.key_pages, cache.value_pages, cache.key_scales))
+    assert all(torch.equal(a, b) for a, b in zip(*results))

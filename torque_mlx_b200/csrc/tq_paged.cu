@@ -333,10 +333,11 @@ int tq_paged_append(const tq_paged_kv* kv, const tq_paged_batch* batch, const vo
   if ((uintptr_t)qkv % 16 || (uintptr_t)q_out % 16 || (uintptr_t)cos_table % 16 || (uintptr_t)sin_table % 16)
     return TQ_E_SHAPE;
   const RopeArgs rope{cos_table, sin_table, positions, rotary_dim, interleaved};
+  const tq_paged_batch b = bounded(*batch);
   cudaStream_t s = (cudaStream_t)stream;
-  if (x_dtype == TQ_F16) return launch_append<__half>(*kv, *batch, qkv, qkv_stride, q_heads, rope, q_out, s);
-  if (x_dtype == TQ_BF16) return launch_append<__nv_bfloat16>(*kv, *batch, qkv, qkv_stride, q_heads, rope, q_out, s);
-  return launch_append<float>(*kv, *batch, qkv, qkv_stride, q_heads, rope, q_out, s);
+  if (x_dtype == TQ_F16) return launch_append<__half>(*kv, b, qkv, qkv_stride, q_heads, rope, q_out, s);
+  if (x_dtype == TQ_BF16) return launch_append<__nv_bfloat16>(*kv, b, qkv, qkv_stride, q_heads, rope, q_out, s);
+  return launch_append<float>(*kv, b, qkv, qkv_stride, q_heads, rope, q_out, s);
 }
 
 int tq_paged_dequantize(const tq_paged_kv* kv, const int32_t* ids, int64_t n, void* k_out, void* v_out,

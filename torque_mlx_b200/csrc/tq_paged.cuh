@@ -67,6 +67,14 @@ inline int check_paged_batch(const tq_paged_batch* b) {
   return TQ_OK;
 }
 
+// The batch with no more rows announced for a sequence than there are: what
+// sizes a launch stays within its types, however large the announced number.
+inline tq_paged_batch bounded(const tq_paged_batch& batch) {
+  tq_paged_batch b = batch;
+  if (b.max_new_tokens > b.rows) b.max_new_tokens = (int32_t)b.rows;
+  return b;
+}
+
 constexpr int kMaxDevices = 64;
 inline int device_index() {
   int dev = 0;

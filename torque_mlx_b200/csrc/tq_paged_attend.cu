@@ -615,12 +615,12 @@ int tq_paged_attend(const tq_paged_kv* kv, const tq_paged_batch* batch, const vo
   if (batch->seqs == 0 || batch->rows == 0 || batch->max_new_tokens == 0) return TQ_OK;
   if (!q || !out) return TQ_E_ARG;
   if ((uintptr_t)q % 16 || (uintptr_t)out % 32) return TQ_E_SHAPE;
-  size_t need = 0;
+  size_t need = 0;  // for the announced rows: the kernel for many needs the most
   tq_paged_attend_workspace_size(kv, q_heads, batch->max_new_tokens, &need);
   if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 32) return TQ_E_WORKSPACE;
   AttendArgs a = {};
   a.kv = *kv;
-  a.bt = *batch;
+  a.bt = bounded(*batch);
   a.q = q;
   a.out = out;
   a.lse = lse;
@@ -631,8 +631,8 @@ int tq_paged_attend(const tq_paged_kv* kv, const tq_paged_batch* batch, const vo
   a.scale2 = scale * 1.44269504f;
   a.part_o = (float*)workspace;
   cudaStream_t s = (cudaStream_t)stream;
-  if (many_rows(batch->max_new_tokens, a.group)) return launch_prefill(a, q_dtype, max_context, s);
-  const int nt = attend_nt(batch->max_new_tokens, a.group);
+  if (many_rows(a.bt.max_new_tokens, a.group)) return launch_prefill(a, q_dtype, max_context, s);
+  const int nt = attend_nt(a.bt.max_new_tokens, a.group);
   a.ctas = attend_ctas(kv->head_dim, nt);
   a.part_l = a.part_o + (size_t)a.ctas * 2 * 8 * nt * kv->head_dim;
   return q_dtype == TQ_F16 ? launch_dim<__half>(a, nt, max_context, s) : launch_dim<__nv_bfloat16>(a, nt, max_context, s);
