@@ -194,3 +194,14 @@ def test_refusals():
     with pytest.raises(ValueError):
         tq.quantize_w4(torch.zeros(4, 4, dtype=torch.int32, device="cuda"))
     assert tq.gemv_w4(w, x[:0]).shape == (0, 32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_infinite_weights_keep_their_sign(dtype):
+    w = torch.randn(3, 64, device="cuda").to(dtype)
+    w[0, 3], w[0, 4], w[0, 5] = math.inf, -math.inf, math.nan
+    packed, scales = tq.quantize_w4(w, group_size=32)
+    codes = torch.stack([packed & 15, packed >> 4], -1).flatten(-2)
+    assert codes[0, 3:6].tolist() == [15, 0, 8]
+    assert bool(torch.isfinite(scales).all())
+    assert torch.equal(packed[1:], tq.quantize_w4(w[1:], group_size=32)[0])

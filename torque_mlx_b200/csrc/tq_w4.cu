@@ -494,7 +494,8 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const T* __restrict__ 
     for (int h = 0; h < 2; ++h) {
       const int64_t col = k0 + 2 * i + h;
       int q = 8;
-      if (col < k) q = min(15, max(0, __float2int_rn(__fdiv_rn(to_f32<T>(w[row * k + col]), s)) + 8));
+      // within [-8, 7] before 8 is added: an infinity converts to the largest integer
+      if (col < k) q = min(7, max(-8, __float2int_rn(__fdiv_rn(to_f32<T>(w[row * k + col]), s)))) + 8;
       byte |= (uint32_t)q << (4 * h);
     }
     if (k0 + 2 * i < k) packed[row * row_bytes + (k0 / 2) + i] = (uint8_t)byte;
