@@ -399,7 +399,12 @@ typedef struct tq_paged_batch {
  * finite scale), scale' = max(amax * fl(1/127), 2^-120, old ? scale : 0).
  * Held tokens become round(code * (scale / scale')) and new ones
  * round(x / scale') within [-127, 127] (a NaN becomes zero), both rounded to
- * even, so a page's codes do not depend on the order of the work. */
+ * even, so a page's codes do not depend on the order of the work.  A page that
+ * holds tokens never goes back to a smaller scale: rows that the caller then
+ * drops (by not counting them in the lengths, as rejected drafts) may have
+ * raised it, and the tokens held keep the coarser codes, each value within half
+ * of the new scale of what it was.  A page whose first tokens are dropped
+ * starts anew. */
 int tq_paged_append(const tq_paged_kv* kv, const tq_paged_batch* batch, const void* qkv, int x_dtype,
                     int64_t qkv_stride, int q_heads, const float* cos_table, const float* sin_table,
                     int64_t positions, int rotary_dim, int interleaved, void* q_out, tq_stream_t stream);

@@ -14,8 +14,12 @@ verified) or many (a prompt's chunk), mixed freely in a batch:
 
 ``lengths`` counts the tokens held before the step: the append writes behind
 them, and the attention sees the written tokens causally.  Advancing the
-lengths afterwards, by as many tokens as are kept, is the caller's, so drafted
-tokens that are rejected need no undoing.
+lengths afterwards, by as many tokens as are kept, is the caller's: drafted
+tokens that are rejected are simply written over.  They may leave a trace: one
+of larger magnitude than a page's scale covers raises that scale, and the
+tokens that the page held before are rounded again to it (each value stays
+within half of the new scale of what it was).  So drafting is not neutral to
+the last bits of what the cache holds.
 """
 
 from __future__ import annotations

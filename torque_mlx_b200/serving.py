@@ -8,9 +8,10 @@ layer by layer,
     gemv_w4 (RMSNorm fused)  ->  PagedKV8Cache.append  ->  PagedKV8Cache.attend
     gemv_w4 (residual)       ->  gemv_w4 (RMSNorm)     ->  gemv_w4 (SwiGLU, residual)
 
-then the output head and ``verify_drafts``.  Rejected drafts need no undoing:
-the lengths advance by what was accepted, and the next step writes over the
-rest.  Drafts come from the sequence itself: what followed the last occurrence
+then the output head and ``verify_drafts``.  The lengths advance by what was
+accepted, and the next step writes over the rejected rest; a rejected token
+that raised its page's scale leaves the page's tokens rounded to that scale
+(see ``paged``).  Drafts come from the sequence itself: what followed the last occurrence
 of its latest tokens.
 """
 
