@@ -205,3 +205,19 @@ def test_infinite_weights_keep_their_sign(dtype):
     assert codes[0, 3:6].tolist() == [15, 0, 8]
     assert bool(torch.isfinite(scales).all())
     assert torch.equal(packed[1:], tq.quantize_w4(w[1:], group_size=32)[0])
+
+
+def test_weight_of_buffers_that_do_not_hold_it():
+    """The product reads by the sizes alone, so buffers of other sizes are refused where the weight is made."""
+    w, _ = make_weight(64, 256, 64)
+    again = tq.W4Weight(w.codes, w.scales, 64, 256, 64)
+    x = torch.randn(2, 256, device="cuda").to(torch.bfloat16)
+    assert torch.equal(tq.gemv_w4(again, x), tq.gemv_w4(w, x))
+    for codes, scales, n, k, group in ((w.codes[:-1024], w.scales, 64, 256, 64), (w.codes, w.scales[:-16], 64, 256, 64),
+                                       (w.codes, w.scales, 4096, 256, 64), (w.codes, w.scales, 64, 2560, 64),
+                                       (w.codes, w.scales, 64, 256, 32), (w.codes.cpu(), w.scales, 64, 256, 64),
+                                       (w.codes, w.scales.cpu(), 64, 256, 64), (w.codes, w.scales.float(), 64, 256, 64),
+                                       (torch.zeros(w.codes.numel() + 1, dtype=torch.uint8, device="cuda")[1:], w.scales, 64, 256, 64),
+                                       (w.codes, w.scales, 64, 256, 48), (w.codes, w.scales, 0, 256, 64)):
+        with pytest.raises(ValueError):
+            tq.W4Weight(codes, scales, n, k, group)

@@ -20,9 +20,16 @@ _MODES = {"plain": 0, "f32": 1, "rms": 2, "silu": 3}
 
 
 class W4Weight:
-    """A 4-bit weight ``[n, k]`` laid out for ``gemv_w4``."""
+    """A 4-bit weight ``[n, k]`` laid out for ``gemv_w4``: the codes and scales
+    as tq_w4_layout wrote them (``from_packed`` and ``quantize`` make them)."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, n: int, k: int, group_size: int):
+        for t, name, size in zip((codes, scales), ("codes", "scales"), self._check_sizes(n, k, group_size)):
+            if t.dtype != torch.uint8 or t.numel() != size or not t.is_cuda or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{name} of a weight [{n}, {k}] must be {size} contiguous bytes (uint8) at a 16-byte "
+                                 "boundary on a CUDA device")
+        if scales.device != codes.device:
+            raise ValueError(f"scales must be on {codes.device}")
         self.codes, self.scales = codes, scales
         self.n, self.k, self.group_size = n, k, group_size
         self.device = codes.device
