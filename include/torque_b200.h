@@ -348,7 +348,10 @@ int tq_gemv(const void* weight, const void* x, int x_mode, const void* norm_weig
  *   k_pages, v_pages   [num_pages, kv_heads, page_size, head_dim] one-byte
  *                      codes biased by 128 (1..255 stand for -127..127),
  *                      16-byte aligned
- *   k_scales, v_scales [num_pages, kv_heads] fp32; value = scale * (code - 128)
+ *   k_scales, v_scales [num_pages, kv_heads] fp32; value = scale * (code - 128).
+ *                      The scales of pages in use are 0 or more, as the append
+ *                      leaves them: the attention takes a negative k scale for
+ *                      a missing page.
  * A batch is ragged: sequence s holds lengths[s] tokens, brings rows
  * [token_starts[s], token_starts[s+1]) of the call's row tensors (row s alone
  * when token_starts is NULL) at positions lengths[s], lengths[s]+1, ..., and

@@ -93,3 +93,15 @@ def test_row_counts_announced_beyond_the_rows():
                                    out.data_ptr(), None, ws.data_ptr(), need.value, stream) == 0
         results.append((q, out, cache.key_pages, cache.value_pages, cache.key_scales))
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("rows", [2, 60])
+def test_a_page_of_negative_key_scale_is_not_attended(rows):
+    """As the header has it, in either kernel: what such a page holds is seen no more than a missing page."""
+    lens, new = [100], [rows]
+    cache, table = make_cache(84, lens, new, page=16, kv_heads=1, d=64)
+    cache.key_scales[table[0, 2].long()] *= -1
+    q = torch.randn(rows, 2, 64, device="cuda").to(torch.bfloat16)
+    got = cache.attend(q, block_table=table, **batch_args(lens, new))
+    table[0, 2] = -1
+    assert torch.equal(got, cache.attend(q, block_table=table, **batch_args(lens, new)))

@@ -730,6 +730,7 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
           if (id >= 0) {
             ks = a.kv.k_scales[block];
             lv = log2f(a.kv.v_scales[block]);
+            if (ks < 0.f) lv = -INFINITY;  // a negative one stands for no page
           }
           if (use > 0 && !(ok = warp_wait(page_empty + 8 * age, (use - 1) & 1))) break;
           if (lane < 8) {

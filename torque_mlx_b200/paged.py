@@ -65,7 +65,8 @@ class PagedKV8Cache:
                    value_scales: torch.Tensor) -> "PagedKV8Cache":
         """Cache over existing buffers, which it shares: codes ``[num_pages,
         kv_heads, page_size, d]`` uint8 (biased by 128) and scales ``[num_pages,
-        kv_heads]`` fp32."""
+        kv_heads]`` fp32.  The scales of pages in use must be 0 or more: a page
+        of negative key scale is not attended."""
         _lib.load()
         for t, name in ((key_pages, "key_pages"), (value_pages, "value_pages")):
             if t.dtype != torch.uint8 or t.dim() != 4 or not t.is_cuda or not t.is_contiguous():
