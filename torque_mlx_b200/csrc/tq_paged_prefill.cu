@@ -4,10 +4,12 @@
 // Mathematics: as in tq_paged_attend.cu, with one exponential for each score.
 // For a page of 2^lv scale, w_j = 2^(s_j + lv - m2) weighs v's codes, and the
 // softmax's own sum l = sum_j 2^(s_j - m), whose reference m is kept apart as
-// there, takes a chunk of one page as (sum_j w_j) 2^(m2 - m - lv).  Where that
-// factor is past 2^64 (the row has seen values so much larger that a chunk's w
-// may vanish before its share of l does) or the page's values have no scale at
-// all, the chunk's own exponentials are taken instead.
+// there, takes a chunk of one page as (sum_j w_j) 2^-lv 2^(m2 - m).  That holds
+// while neither factor leaves fp32's range and no w vanishes before its share of
+// l does: up to 2^60 for m2 - m and 2^40 for m2 - m - lv of every page of a step
+// (s - m then stays under 55).  Where a row is past that, among pages 2^40 apart
+// in scale or beside one whose values have none, the step's scores are summed
+// by themselves.
 //
 // Bound: the two products, 4 d flops for each visible (row, token) pair, on
 // the tensor cores, and the exponentials, which take as long at d = 128 (16 a
@@ -24,9 +26,11 @@
 // Each half has two score buffers, so the next step's scores are ready when a
 // softmax ends, whatever the other half does.
 //
-// Measured: 972 tokens behind 4099, 16 heads over 8 of 128: 69 us, 0.53 PFLOP/s.
-// Within a unit a tile of 256 rows by 128 tokens takes 2.3 us (1.08 PFLOP/s over
-// the card); the query rows take 5 us a unit, the output 4, the join 8.
+// Measured: 972 tokens behind 4099, 16 heads over 8 of 128: 72 us, 0.51 PFLOP/s
+// (over 8 of 64: 59 us, over 2 of 256: 122 us).  Within a unit a tile of 256
+// rows by 128 tokens takes 2.4 us (1.04 PFLOP/s over the card, 2.35 us without a
+// reference of l's own); the query rows take 5 us a unit, the output 4, the
+// join 8.
 #include <atomic>
 
 #include "tq_paged_attend.cuh"
@@ -37,8 +41,9 @@ constexpr int kRows = 128;          // query rows of a product
 constexpr int kTokens = 128;        // tokens of a tile
 constexpr int kStep = 64;           // tokens of a step
 // What a unit costs besides its tiles (its query rows, the output), in tiles.
-// 972 tokens alone take 40 us with 0, 38 with 2, 35 with 3, 34 with 5; behind
-// 4099 tokens 74, 72, 69, 70; 20 chunks of up to 64 tokens 75 with 2, 72 with 3.
+// 972 tokens alone take 41 us with 0, 39 with 2, 36 with 3, 36 with 5; behind
+// 4099 tokens 79, 75, 73, 74; 20 chunks of up to 64 tokens over up to 3000 43,
+// 35, 31, 32.
 constexpr int kPrefillLead = 3;
 constexpr int kPrefillShare = 2;    // smallest share of a CTA, in tiles
 
@@ -244,24 +249,27 @@ __device__ __forceinline__ uint32_t place(int t, int q) { return (uint32_t)((q >
 
 // A step's chunks of sixteen tokens as the softmax uses them: products times f
 // are the scores, and with the logarithm of v's scale the weights' exponents.
-// Without a page f is negative and the logarithm -inf.
+// inv is v's scale inverted.  Without a page f is negative, the logarithm -inf
+// and inv 0.
 struct StepScales {
-  float f[4], lv[4];
+  float f[4], lv[4], inv[4];
 
-  __device__ __forceinline__ StepScales(const float* ks, const float* lvs, float kf) {
-    const float4 k = *reinterpret_cast<const float4*>(ks), v = *reinterpret_cast<const float4*>(lvs);
+  __device__ __forceinline__ StepScales(const float* ks, const float* lvs, const float* invs, float kf) {
+    const float4 k = *reinterpret_cast<const float4*>(ks), v = *reinterpret_cast<const float4*>(lvs),
+                 i = *reinterpret_cast<const float4*>(invs);
     f[0] = k.x, f[1] = k.y, f[2] = k.z, f[3] = k.w;
     lv[0] = v.x, lv[1] = v.y, lv[2] = v.z, lv[3] = v.w;
+    inv[0] = i.x, inv[1] = i.y, inv[2] = i.z, inv[3] = i.w;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       if (f[c] >= 0.f) f[c] *= kf;
   }
 };
 
-// The largest exponent of a row's step, and its largest score; columns past
-// `seen` are hidden where MASKED.
-template <bool MASKED>
-__device__ __forceinline__ float highest(const float (&v)[kStep], const StepScales& w, int seen, float& score) {
+// The largest exponent of a row's step, or its largest score where SCORE;
+// columns past `seen` are hidden where MASKED.
+template <bool MASKED, bool SCORE>
+__device__ __forceinline__ float highest(const float (&v)[kStep], const StepScales& w, int seen) {
   float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int k = 0; k < 16; ++k)
@@ -269,43 +277,30 @@ __device__ __forceinline__ float highest(const float (&v)[kStep], const StepScal
     for (int c = 0; c < 4; ++c)
       if (!MASKED || c * 16 + k <= seen) x[c] = fmaxf(x[c], v[c * 16 + k]);
   // a NaN (nothing visible, or no page) is passed over
-  float s[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    s[c] = w.f[c] < 0.f ? -INFINITY : x[c] * w.f[c];
-    x[c] = fmaf(x[c], w.f[c], w.lv[c]);
+    if (SCORE) x[c] = w.f[c] < 0.f ? -INFINITY : x[c] * w.f[c];
+    else x[c] = fmaf(x[c], w.f[c], w.lv[c]);
   }
-  score = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
   return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
 }
 
-// sum_j 2^(s_j - m) of chunk c
+// l and its reference m after a step whose scores are summed by themselves.
 template <bool MASKED>
-__device__ __forceinline__ float chunk_sum(const float (&v)[kStep], const StepScales& w, int c, float m, int seen) {
-  float sum = 0.f;
+__device__ __forceinline__ void sum_scores(const float (&v)[kStep], const StepScales& w, int seen, float& m, float& l) {
+  const float nm = fmaxf(m, highest<MASKED, true>(v, w, seen));
+  l *= ex2(m - nm);
+  m = nm;
 #pragma unroll
-  for (int k = 0; k < 16; ++k)
-    if (!MASKED || c * 16 + k <= seen) sum += ex2(fmaf(v[c * 16 + k], w.f[c], -m));
-  return sum;
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (w.f[c] >= 0.f && (!MASKED || c * 16 + k <= seen)) l += ex2(fmaf(v[c * 16 + k], w.f[c], -m));
 }
 
-// The row's weights to tensor memory, and the sum of 2^(s - m) to l.
+// The row's weights to tensor memory; returns the sum of 2^(s - m2).
 template <bool MASKED>
-__device__ __forceinline__ void weigh(uint32_t at, const float (&v)[kStep], const StepScales& w, float m, float m2, int seen,
-                                      float& l) {
-  float factor[4];
-  bool apart = false;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const float e = m2 - m - w.lv[c];
-    factor[c] = w.f[c] < 0.f || e > 64.f ? 0.f : ex2(e);
-    apart |= w.f[c] >= 0.f && e > 64.f;
-  }
-  if (__any_sync(FULL, apart)) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-      if (w.f[c] >= 0.f && m2 - m - w.lv[c] > 64.f) l += chunk_sum<MASKED>(v, w, c, m, seen);
-  }
+__device__ __forceinline__ float weigh(uint32_t at, const float (&v)[kStep], const StepScales& w, float m2, int seen) {
   float sums[4];
 #pragma unroll
   for (int b = 0; b < 2; ++b) {
@@ -344,7 +339,7 @@ __device__ __forceinline__ void weigh(uint32_t at, const float (&v)[kStep], cons
       sums[2 * b + u] = e.x + e.y;
     }
   }
-  l += fmaf(sums[0], factor[0], sums[1] * factor[1]) + fmaf(sums[2], factor[2], sums[3] * factor[3]);
+  return fmaf(sums[0], w.inv[0], sums[1] * w.inv[1]) + fmaf(sums[2], w.inv[2], sums[3] * w.inv[3]);
 }
 
 // A part of a unit that falls to a CTA.
@@ -417,9 +412,11 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
   __shared__ uint32_t tmem_at;
   __shared__ volatile int failed;
   // of a tile's chunks of sixteen tokens: page and head (page 0 and a k scale of
-  // -1 where there is none), k's scale and the logarithm of v's
+  // -1 where there is none), k's scale, the logarithm and the inverse of v's, and
+  // of a step's chunks the smallest logarithm
   __shared__ uint32_t page_at[Shape::kAges][8];
-  __shared__ __align__(16) float page_k[Shape::kAges][8], page_lv[Shape::kAges][8];
+  __shared__ __align__(16) float page_k[Shape::kAges][8], page_lv[Shape::kAges][8], page_inv[Shape::kAges][8];
+  __shared__ float page_low[Shape::kAges][2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t raw = (uint32_t)__cvta_generic_to_shared(prefill_smem), base = (raw + 1023u) & ~1023u;
   uint8_t* const smem = prefill_smem + (base - raw);
@@ -559,40 +556,51 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
           const uint32_t buf = j & 1, ph = (pairs_done + (j >> 1)) & 1, age = (tiles_done + (j >> 1)) % Shape::kAges;
           if (!(ok = warp_wait(s_done + 8 * (2 * half + buf), ph))) break;
           tc_fence_after();
-          const StepScales scales(page_k[age] + 4 * buf, page_lv[age] + 4 * buf, kf);
+          const StepScales scales(page_k[age] + 4 * buf, page_lv[age] + 4 * buf, page_inv[age] + 4 * buf, kf);
+          const float low = page_low[age][buf];
           float v[kStep];
           tmem_load64(t_half + buf * kStep, v);
           const int tok = u.c0 * kTokens + j * kStep;
           const bool masked = tok + kStep - 1 > free_to;
           const int seen = limit - tok;  // columns 0..seen are visible
-          float score;
-          const float top = masked ? highest<true>(v, scales, seen, score) : highest<false>(v, scales, seen, score);
-          if (__any_sync(FULL, top > m2 + (kLazy + kRoom) || score > m + kLazy)) {
-            const float nm = fmaxf(m, score), nm2 = fmaxf(m2, top - kRoom), f = ex2(m2 - nm2);
-            l *= ex2(m - nm);
-            m = nm;
-            m2 = nm2;
-            if (j > 0 && __any_sync(FULL, f != 1.f)) {  // the sums of the steps before, once their products are complete
-              if (!(ok = warp_wait(pv_done + 8 * (2 * half + 1 - buf), (pairs_done + ((j - 1) >> 1)) & 1))) break;
-              tc_fence_after();
+          const float top = masked ? highest<true, false>(v, scales, seen) : highest<false, false>(v, scales, seen);
+          bool apart = false;
+          // one vote while the references hold and l can be taken from the weights
+          if (__any_sync(FULL, top > m2 + (kLazy + kRoom) || fabsf(m2 - m) > 60.f || m2 - m - low > 40.f)) {
+            if (__any_sync(FULL, top > m2 + (kLazy + kRoom))) {
+              const float score = masked ? highest<true, true>(v, scales, seen) : highest<false, true>(v, scales, seen);
+              const float nm = fmaxf(m, score), nm2 = fmaxf(m2, top - kRoom), f = ex2(m2 - nm2);
+              l *= ex2(m - nm);
+              m = nm;
+              m2 = nm2;
+              if (j > 0) {  // the sums of the steps before, once their products are complete
+                if (!(ok = warp_wait(pv_done + 8 * (2 * half + 1 - buf), (pairs_done + ((j - 1) >> 1)) & 1))) break;
+                tc_fence_after();
 #pragma unroll 1
-              for (int b = 0; b < D / 16; ++b) {
-                uint32_t x[16];
-                asm volatile(
-                    "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                    "\n\ttcgen05.wait::ld.sync.aligned;"
-                    : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]),
-                      "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
-                    : "r"(t_o + b * 16)
-                    : "memory");
+                for (int b = 0; b < D / 16; ++b) {
+                  uint32_t x[16];
+                  asm volatile(
+                      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                      "\n\ttcgen05.wait::ld.sync.aligned;"
+                      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]),
+                        "=r"(x[8]), "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+                      : "r"(t_o + b * 16)
+                      : "memory");
 #pragma unroll
-                for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
-                tmem_store16(t_o + b * 16, x);
+                  for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
+                  tmem_store16(t_o + b * 16, x);
+                }
               }
             }
+            apart = __any_sync(FULL, fabsf(m2 - m) > 60.f || m2 - m - low > 40.f);
+            if (apart) {
+              if (masked) sum_scores<true>(v, scales, seen, m, l);
+              else sum_scores<false>(v, scales, seen, m, l);
+            }
           }
-          if (masked) weigh<true>(t_half + buf * kStep, v, scales, m, m2, seen, l);
-          else weigh<false>(t_half + buf * kStep, v, scales, m, m2, seen, l);
+          const float sum = masked ? weigh<true>(t_half + buf * kStep, v, scales, m2, seen)
+                                   : weigh<false>(t_half + buf * kStep, v, scales, m2, seen);
+          if (!apart) l = fmaf(sum, ex2(m2 - m), l);
           tmem_store_wait();
           tc_fence_before();
           bar_arrive(p_full + 8 * (2 * half + buf));
@@ -732,11 +740,16 @@ __global__ void __launch_bounds__(PrefillShape<D>::kThreads, 1) paged_prefill_ke
             lv = log2f(a.kv.v_scales[block]);
             if (ks < 0.f) lv = -INFINITY;  // a negative one stands for no page
           }
+          float low = ks < 0.f ? INFINITY : lv;
+          low = fminf(low, __shfl_xor_sync(FULL, low, 1));
+          low = fminf(low, __shfl_xor_sync(FULL, low, 2));
           if (use > 0 && !(ok = warp_wait(page_empty + 8 * age, (use - 1) & 1))) break;
           if (lane < 8) {
             page_at[age][lane] = (uint32_t)block;
             page_k[age][lane] = ks;
             page_lv[age][lane] = lv;
+            page_inv[age][lane] = ks < 0.f ? 0.f : ex2(-lv);
+            if ((lane & 3) == 0) page_low[age][lane >> 2] = low;
           }
           __syncwarp();
           bar_arrive(page_full + 8 * age);
