@@ -9,9 +9,11 @@
 // for each page and head means no atomics, so the codes are the same for
 // every run, and one launch covers q, k and v.
 //
-// Measured: one token of each of 64 sequences, 32 + 2 x 8 heads of 128: 10.5 us
-// (26.6 MB, 2.5 TB/s); 7 prompts of up to 1531 tokens, 16 + 2 x 2 heads of 256:
-// 33 us (135 MB, 4.1 TB/s).
+// Measured within a graph: one token of each of 64 sequences, 32 + 2 x 8 heads of
+// 128: 4.4 us (1.4 MB: dependent loads bound it), and 6.0 for the values of their
+// 64 last pages (25 MB); 7 prompts of 7197 tokens, 16 + 2 x 2 heads of 256: 35 us
+// (140 MB, 4.0 TB/s: no load of a next page is in flight while a CTA reduces its
+// maximum).
 #include "tq_paged.cuh"
 
 namespace tq {
@@ -288,11 +290,13 @@ int launch_append(const tq_paged_kv& kv, const tq_paged_batch& b, const void* qk
   const int pages = (b.max_new_tokens + kv.page_size - 2) / kv.page_size + 1;
   const int64_t x = (int64_t)b.seqs * pages;
   if (x > INT32_MAX || kv.kv_heads > 65535) return TQ_E_SHAPE;
-  // 128 threads while a page gains few tokens (one token of 64 sequences: 10.5
-  // us, 17.2 with 256), 256 for prompts (7 of up to 1531 tokens: 32.9 us, 33.7
-  // with 128).  The q heads of a kv head share a CTA (and the angles a thread
-  // loads) up to sixteen items a thread: 2, 4, 8 and 16 take 42.7, 38.3, 33.3
-  // and 33.0 us for the same prompts.
+  // 128 threads while a page gains few tokens (one token of 64 sequences: 4.4 us,
+  // 11.0 with 256), 256 for prompts, whose pages of up to 64 x 128 they hold in
+  // registers between the passes (prompts of 7197 tokens in pages of 32 x 256
+  // take 34.6 us, and 31.2 with 128 threads, so the rule is not the best there).
+  // The q heads of a kv head share a CTA (and the angles a thread loads) up to
+  // sixteen items a thread: 2, 4, 8 and 16 take 42.4, 37.9, 32.5 and 34.6 us for
+  // the same prompts.
   const int rows = b.max_new_tokens < kv.page_size ? b.max_new_tokens : kv.page_size, items = rows * (kv.head_dim / 16);
   const int group = q_heads / kv.kv_heads;
   const bool wide = items > 128;

@@ -93,7 +93,10 @@ inline int sm_count() {
 }
 
 // Launch that may begin while the stream's previous kernel drains: every CTA
-// of the kernel runs griddepcontrol.wait before it touches memory.
+// of the kernel runs griddepcontrol.wait before it touches memory that a kernel
+// before it may still write.  The attentions' joins read the batch's lengths and
+// row starts before that, to plan while the attention runs: its CTAs let them
+// start only after their own wait, which covers what wrote those.
 template <typename... P, typename... A>
 inline int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
   cudaLaunchConfig_t cfg = {};

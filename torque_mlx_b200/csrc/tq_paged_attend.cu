@@ -570,9 +570,17 @@ int launch_dim(const AttendArgs& a, int nt, int64_t max_context, cudaStream_t st
   return launch_rows<256, T>(a, nt, max_context, stream);
 }
 
-// Query rows of a kv head from which on the tiles of 128 rows take over: 8
-// sequences of 4000 tokens and 8 heads take 40 us with 24 rows and 44 with 32
-// in tiles of 16, and 52 with 33 to 64 in tiles of 128.
+// Query rows of a kv head from which on the tiles of 128 rows take over.  8
+// sequences and 8 heads of 128, in tiles of 16 and of 128:
+//   rows    1000 tokens   4000 tokens   32000 tokens
+//   32      20.4  26.5    39.3  47.2
+//   40      25.7  27.0    53.2  47.2    304  236
+//   41      25.9  27.0    53.5  47.6    305  238
+//   64      31.3  27.8    68.6  48.4    408  237
+// so from 33 rows on long contexts would gain already, and short ones lose.  The
+// count is the largest one of the batch: sequences of one token beside a chunk
+// go the chunk's way, which costs them (63 over 4000 tokens with a chunk of 512,
+// 32 heads over 8: 405 us in one call, 89 and 69 apart).
 constexpr int kPrefillFrom = 41;
 inline bool many_rows(int64_t max_new, int group) { return max_new * group >= kPrefillFrom; }
 

@@ -41,9 +41,9 @@ constexpr int kRows = 128;          // query rows of a product
 constexpr int kTokens = 128;        // tokens of a tile
 constexpr int kStep = 64;           // tokens of a step
 // What a unit costs besides its tiles (its query rows, the output), in tiles.
-// 972 tokens alone take 41 us with 0, 39 with 2, 36 with 3, 36 with 5; behind
-// 4099 tokens 79, 75, 73, 74; 20 chunks of up to 64 tokens over up to 3000 43,
-// 35, 31, 32.
+// 972 tokens alone take 41 us with 0, 39 with 2, 37 with 3, 36 with 5; behind
+// 4099 tokens 77, 75, 72, 73; 20 chunks of up to 64 tokens over up to 3000 43,
+// 35, 32, 32.
 constexpr int kPrefillLead = 3;
 constexpr int kPrefillShare = 2;    // smallest share of a CTA, in tiles
 
