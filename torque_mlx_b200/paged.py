@@ -106,7 +106,8 @@ class PagedKV8Cache:
         return the rotated queries ``[rows, q_heads, d]`` (tq_paged_append).
 
         ``qkv`` is ``[rows, (q_heads + 2 kv_heads) * d]`` (fp16, bf16 or fp32,
-        row stride free); rows ``token_starts[s]`` to ``token_starts[s + 1]``
+        row stride free; the queries come back in its type, of which ``attend``
+        takes fp16 and bf16); rows ``token_starts[s]`` to ``token_starts[s + 1]``
         belong to sequence ``s`` (row ``s`` without ``token_starts``) and take
         the positions from ``lengths[s]`` on.  ``cos`` / ``sin`` are fp32
         ``[positions, rotary_dim / 2]`` tables; pairs are ``(2i, 2i + 1)``, or
